@@ -8,6 +8,7 @@
 #include <vector>
 
 #include "../../include/mimo_moe_layer.h"
+#include "../../include/mimo_moe_paged.h"
 #include "common.cuh"
 #include "kernels.h"
 
@@ -1135,6 +1136,91 @@ int mimo_moe_layer_swiglu(const uint16_t* gate_up, int32_t T, int32_t I, uint16_
 int mimo_moe_layer_add(const uint16_t* a, const uint16_t* b, int64_t n, uint16_t* out, void* stream) {
   if (!a || !b || !out || n < 8 || n % 8 || !a16(a) || !a16(b) || !a16(out)) return MIMO_EINVAL;
   MIMO_TRY(launch_add(a, b, (size_t)n, out, static_cast<cudaStream_t>(stream)));
+  return MIMO_OK;
+}
+
+// ------------------------------------------------------------------ paged serving (include/mimo_moe_paged.h)
+namespace {
+constexpr int kMaxRequests = 4096;
+int page_shift_of(int32_t page_size) {  // log2 of a supported page size, else -1
+  for (int s = 4; s <= 7; ++s)
+    if (page_size == 1 << s) return s;
+  return -1;
+}
+bool bad_pool(int32_t num_pages, int32_t page_size) {  // slot numbers are int32
+  return num_pages < 1 || page_shift_of(page_size) < 0 || (int64_t)num_pages * page_size > INT32_MAX;
+}
+bool bad_table(int32_t R, int32_t width, int32_t page_size) {  // positions are int32
+  return R < 1 || R > kMaxRequests || width < 1 || (int64_t)width * page_size > INT32_MAX;
+}
+}  // namespace
+
+int mimo_moe_page_plan(const int32_t* lens, const int32_t* new_lens, int32_t R, int32_t* block_table,
+                       int32_t table_width, const int32_t* free_pages, const int32_t* n_free, int32_t num_pages,
+                       int32_t page_size, int32_t tokens, int32_t* cu_q, int32_t* seq_lens, int32_t* n_free_out,
+                       int32_t* positions, int32_t* slots, int32_t* status, void* stream) {
+  if (!lens || !new_lens || !block_table || !free_pages || !n_free || !cu_q || !seq_lens || !n_free_out ||
+      (tokens > 0 && (!positions || !slots)) || tokens < 0 || bad_pool(num_pages, page_size) ||
+      bad_table(R, table_width, page_size) || seq_lens == lens || seq_lens == new_lens || n_free_out == n_free)
+    return MIMO_EINVAL;
+  PagePlanParams p{};
+  p.lens = lens, p.new_lens = new_lens, p.table = block_table, p.free_pages = free_pages, p.n_free = n_free;
+  p.cu_q = cu_q, p.seq_lens = seq_lens, p.n_free_out = n_free_out, p.positions = positions, p.slots = slots;
+  p.status = status, p.R = R, p.width = table_width, p.num_pages = num_pages, p.page_shift = page_shift_of(page_size);
+  p.tokens = tokens;
+  MIMO_TRY(launch_page_plan(p, static_cast<cudaStream_t>(stream)));
+  return MIMO_OK;
+}
+
+int mimo_moe_page_release(const uint8_t* done, int32_t R, int32_t* lens, int32_t* block_table, int32_t table_width,
+                          int32_t* free_pages, int32_t* n_free, int32_t num_pages, int32_t page_size,
+                          int32_t* status, void* stream) {
+  if (!done || !lens || !block_table || !free_pages || !n_free || bad_pool(num_pages, page_size) ||
+      bad_table(R, table_width, page_size))
+    return MIMO_EINVAL;
+  PageReleaseParams p{};
+  p.done = done, p.lens = lens, p.table = block_table, p.free_pages = free_pages, p.n_free = n_free;
+  p.status = status, p.R = R, p.width = table_width, p.num_pages = num_pages, p.page_shift = page_shift_of(page_size);
+  MIMO_TRY(launch_page_release(p, static_cast<cudaStream_t>(stream)));
+  return MIMO_OK;
+}
+
+int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                              int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,
+                              float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
+                              int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages, int32_t* status,
+                              void* stream) {
+  if (!qkv || !positions || !slots || !q || !k_pages || !v_pages || tokens < 1 || n_heads < 1 || n_kv_heads < 1 ||
+      head_dim < 8 || v_head_dim < 8 || head_dim % 8 || v_head_dim % 8 || rotary_dim < 0 || rotary_dim % 2 ||
+      rotary_dim > head_dim || rotary_dim > 256 || !(rope_theta > 0.f) || !(v_scale >= 0.f) ||
+      bad_pool(num_pages, page_size) || !a16(qkv) || !a16(q) || !a16(k_pages) || !a16(v_pages))
+    return MIMO_EINVAL;
+  PagedRopeParams p{};
+  p.qkv = qkv, p.positions = positions, p.slots = slots, p.q = q, p.k = k_pages, p.v = v_pages, p.status = status;
+  p.T = tokens, p.nq = n_heads, p.nkv = n_kv_heads, p.dqk = head_dim, p.dv = v_head_dim, p.rot = rotary_dim;
+  p.num_pages = num_pages, p.page_shift = page_shift_of(page_size), p.has_vscale = v_scale > 0.f ? 1 : 0;
+  p.v_scale = v_scale, p.log_base = std::log((double)rope_theta);
+  MIMO_TRY(launch_paged_rope(p, static_cast<cudaStream_t>(stream)));
+  return MIMO_OK;
+}
+
+int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
+                             const int32_t* block_table, int32_t table_width, const int32_t* cu_q,
+                             const int32_t* seq_lens, int32_t R, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                             int32_t head_dim, int32_t v_head_dim, float scale, int32_t window, int32_t keep_first,
+                             int32_t num_pages, int32_t page_size, uint16_t* out, int32_t* status, void* stream) {
+  if (!q || !k_pages || !v_pages || !block_table || !cu_q || !seq_lens || !out || tokens < 1 || n_heads < 1 ||
+      n_kv_heads < 1 || n_heads % n_kv_heads || n_heads / n_kv_heads > 128 ||
+      !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 || keep_first < 0 ||
+      (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) || bad_table(R, table_width, page_size) ||
+      !a16(q) || !a16(k_pages) || !a16(v_pages) || !a16(out))
+    return MIMO_EINVAL;
+  PagedAttnParams p{};
+  p.q = q, p.k = k_pages, p.v = v_pages, p.sinks = sinks, p.table = block_table, p.cu_q = cu_q, p.seq_lens = seq_lens;
+  p.out = out, p.status = status, p.T = tokens, p.R = R, p.width = table_width, p.nq = n_heads, p.nkv = n_kv_heads;
+  p.dqk = head_dim, p.dv = v_head_dim, p.window = window, p.keep = keep_first, p.num_pages = num_pages;
+  p.page_shift = page_shift_of(page_size), p.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  MIMO_TRY(launch_paged_attention(p, static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
 }
 

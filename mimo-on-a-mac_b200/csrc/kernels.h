@@ -322,4 +322,40 @@ cudaError_t launch_add_rmsnorm(const uint16_t* x, const uint16_t* d, const uint1
 cudaError_t launch_swiglu(const uint16_t* gu, int T, int I, uint16_t* out, cudaStream_t st);
 cudaError_t launch_add(const uint16_t* a, const uint16_t* b, size_t n, uint16_t* out, cudaStream_t st);
 
+// ---- many requests over a paged KV cache (paged.cu, paged_attn.cu)
+struct PagePlanParams {
+  const int32_t *lens, *new_lens;  // [R]
+  int32_t* table;                  // [R][width] page numbers
+  const int32_t *free_pages, *n_free;
+  int32_t *cu_q, *seq_lens, *n_free_out, *positions, *slots, *status;
+  int R, width, num_pages, page_shift, tokens;
+};
+struct PageReleaseParams {
+  const uint8_t* done;  // [R]
+  int32_t *lens, *table, *free_pages, *n_free, *status;
+  int R, width, num_pages, page_shift;
+};
+struct PagedRopeParams {
+  const uint16_t* qkv;               // [T][nq*dqk + nkv*dqk + nkv*dv] projection rows
+  const int32_t *positions, *slots;  // [T], slot -1: not a token
+  uint16_t *q, *k, *v;               // q [T][nq][dqk], pools [num_pages][nkv][page][d]
+  int32_t* status;
+  int T, nq, nkv, dqk, dv, rot, num_pages, page_shift, has_vscale;
+  float v_scale;    // already a bf16 value
+  double log_base;  // ln(rope_theta)
+};
+struct PagedAttnParams {
+  const uint16_t *q, *k, *v;   // q [T][nq][dqk], pools [num_pages][nkv][page][d]
+  const float* sinks;          // [nq] sink logits, or null
+  const int32_t *table, *cu_q, *seq_lens;
+  uint16_t* out;               // [T][nq][dv]
+  int32_t* status;
+  int T, R, width, nq, nkv, dqk, dv, window, keep, num_pages, page_shift;
+  float scale_log2;            // softmax scale * log2(e)
+};
+cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st);
+cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st);
+cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st);
+cudaError_t launch_paged_attention(const PagedAttnParams& p, cudaStream_t st);
+
 }  // namespace mimo

@@ -1,4 +1,4 @@
-"""ctypes bindings of libmimo_moe.so (the C ABI in include/mimo_moe.h and include/mimo_moe_layer.h) and of the test and benchmark
+"""ctypes bindings of libmimo_moe.so (the C ABI in include/mimo_moe.h, mimo_moe_layer.h and mimo_moe_paged.h) and of the test and benchmark
 kit beside it, libmimo_moe_testkit.so (include/mimo_moe_testkit.h: synthetic pools, tensor-peak probe).
 
 There is no CPU fallback: if the library is missing or cannot be loaded, every op raises."""
@@ -99,6 +99,16 @@ SIGNATURES = {
                                              c_void_p, c_void_p]),
     "mimo_moe_layer_swiglu": (c_int32, [c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
     "mimo_moe_layer_add": (c_int32, [c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mimo_moe_page_plan": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_int32,
+                                     c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "mimo_moe_page_release": (c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_int32, c_void_p, c_void_p, c_int32,
+                                        c_int32, c_void_p, c_void_p]),
+    "mimo_moe_paged_rope_store": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+                                            c_float, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                                            c_void_p, c_void_p]),
+    "mimo_moe_paged_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p,
+                                           c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float, c_int32,
+                                           c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "mimo_moe_profile_enable": (c_int32, [c_int32]),
     "mimo_moe_profile_read": (c_int32, [c_void_p, c_void_p]),
 }

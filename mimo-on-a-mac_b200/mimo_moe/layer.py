@@ -38,6 +38,7 @@ class AttentionConfig:
     window: int = 0                 # sliding_window_size on SWA layers, 0 = full causal attention
     sinks: bool = False             # add_{full,swa}_attention_sink_bias
     v_scale: Optional[float] = None  # attention_value_scale
+    keep_first: int = 0             # first tokens that stay visible past the window (paged attention only)
 
     @property
     def scale(self) -> float:
@@ -66,6 +67,8 @@ class KVCache:
     position p in slot p % cap.  Full attention: cap = the longest sequence (mlx_lm KVCache); sliding window:
     a ring of window + max_chunk - 1 slots (RotatingKVCache(max_size=window) keeps the last `window` keys and
     concatenates a multi-token chunk before trimming, which is what the extra max_chunk - 1 slots hold)."""
+
+    paged = False   # one sequence, as against mimo_moe.paged.PagedKVCache
 
     def __init__(self, cfg: AttentionConfig, cap: int, device=None):
         dev = torch.device(device or "cuda")
@@ -108,6 +111,8 @@ def attention(q: torch.Tensor, cache: KVCache, cfg: AttentionConfig, pos0: int, 
     rows run on the tcgen05 kernel (cache capacity a multiple of 128), decode-sized calls on the split-key
     mma.sync kernel.  Returns bf16 [T, n_heads, v_head_dim]."""
     _need_cuda(q, "q")
+    if cfg.keep_first:
+        raise ValueError("attention: a ring cache no longer holds the first tokens (keep_first needs a paged cache)")
     q = q.to(torch.bfloat16).contiguous()
     T = q.shape[0]
     dev = q.device
@@ -217,6 +222,8 @@ class Attention:
     def __call__(self, r: torch.Tensor, cache: KVCache) -> torch.Tensor:
         T = r.shape[0]
         cfg = self.cfg
+        if cache.paged:   # rows of many requests, laid out by the cache's step
+            return linear(cache.attend(linear(r, self.w_qkv), self.sinks).view(T, -1), self.w_o)
         # the attention call's own check (every key visible to the chunk still in the ring), made before the
         # cache append so a refused chunk leaves the cache as it was
         first = max(0, cache.offset - cfg.window + 1) if cfg.window > 0 else 0

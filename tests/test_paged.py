@@ -1,0 +1,86 @@
+"""The paged serving operators' refusals (no GPU needed): bad arguments at the C entries before any launch, and the
+Python checks."""
+import pytest
+import torch
+
+EINVAL = 1
+
+
+def _lib():
+    import mimo_moe
+    return mimo_moe.lib()
+
+
+def test_header_is_bound():
+    from test_cabi import declared_functions
+    from mimo_moe._lib import SIGNATURES
+    names = declared_functions("mimo_moe_paged.h")
+    L = _lib()
+    assert names and all(hasattr(L, n) and n in SIGNATURES for n in names)
+
+
+A = 1 << 20   # an aligned address that no refused call touches
+
+
+def plan_args(**kw):
+    d = dict(lens=A, new=A + 64, R=2, table=A, width=4, free=A, n_free=A + 128, pages=8, P=16, T=4, cu=A, seq=A + 256,
+             n_out=A + 512, pos=A, slots=A, status=None, stream=None)
+    d.update(kw)
+    return list(d.values())
+
+
+@pytest.mark.parametrize("bad", [dict(lens=None), dict(new=None), dict(table=None), dict(free=None), dict(n_free=None),
+                                 dict(cu=None), dict(seq=None), dict(n_out=None), dict(pos=None), dict(slots=None),
+                                 dict(R=0), dict(R=4097), dict(width=0), dict(pages=0), dict(P=0), dict(P=8), dict(P=48),
+                                 dict(P=256), dict(T=-1), dict(seq=A), dict(seq=A + 64), dict(n_out=A + 128),
+                                 dict(pages=1 << 28), dict(width=1 << 28)])
+def test_page_plan_refuses(bad):
+    assert _lib().mimo_moe_page_plan(*plan_args(**bad)) == EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(done=None), dict(lens=None), dict(table=None), dict(free=None), dict(n_free=None),
+                                 dict(R=0), dict(R=4097), dict(width=0), dict(pages=0), dict(P=20)])
+def test_page_release_refuses(bad):
+    d = dict(done=A, R=2, lens=A, table=A, width=4, free=A, n_free=A, pages=8, P=16, status=None, stream=None)
+    d.update(bad)
+    assert _lib().mimo_moe_page_release(*d.values()) == EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(qkv=None), dict(q=None), dict(k=None), dict(v=None), dict(pos=None),
+                                 dict(slots=None), dict(T=0), dict(nq=0), dict(nkv=0), dict(d=12), dict(dv=12),
+                                 dict(rot=3), dict(rot=-2), dict(rot=194), dict(d=512, rot=258), dict(theta=0.0),
+                                 dict(vs=-1.0), dict(vs=float("nan")), dict(pages=0), dict(P=100), dict(qkv=A + 8),
+                                 dict(q=A + 2), dict(k=A + 8), dict(v=A + 4)])
+def test_paged_rope_store_refuses(bad):
+    d = dict(qkv=A, T=4, nq=8, nkv=2, d=192, dv=128, rot=64, theta=1e4, vs=0.0, pos=A, slots=A, pages=8, P=16, q=A,
+             k=A, v=A, status=None, stream=None)
+    d.update(bad)
+    assert _lib().mimo_moe_paged_rope_store(*d.values()) == EINVAL
+
+
+def test_python_checks_refuse():
+    from mimo_moe import paged
+    from mimo_moe.layer import AttentionConfig
+    cpu = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        paged.PageStep(block_table=torch.zeros(2, 4, dtype=torch.int32), page_size=16, cu_q=cpu, seq_lens=cpu,
+                       positions=cpu, slots=cpu)
+    with pytest.raises(ValueError):
+        paged.page_plan(cpu, cpu, torch.zeros(2, 4, dtype=torch.int32), cpu, cpu[:1], 16, 4)
+    with pytest.raises(ValueError):
+        paged.page_release(torch.zeros(2, dtype=torch.bool), cpu, torch.zeros(2, 4, dtype=torch.int32), cpu, cpu[:1], 16)
+    for kw in (dict(page_size=24), dict(max_requests=0), dict(max_requests=5000), dict(max_len=0), dict(num_pages=0),
+               dict(num_pages=1 << 28)):
+        with pytest.raises(ValueError):
+            paged.PageTable(**{**dict(max_requests=4, max_len=64, num_pages=8, page_size=16, device="cpu"), **kw})
+    with pytest.raises(ValueError):
+        paged.PagedKVCache(AttentionConfig(), 4, 16, "cpu")
+    with pytest.raises(ValueError):
+        paged.PagedDecoderStack([], 4, 64, 8)
+
+
+def test_ring_attention_refuses_first_tokens_that_stay():
+    from mimo_moe.layer import AttentionConfig, KVCache, attention
+    cfg = AttentionConfig(window=128, keep_first=4)
+    with pytest.raises(ValueError):
+        attention(torch.zeros(1, 64, 192), KVCache(cfg, 128, "cpu"), cfg, 0)
