@@ -67,14 +67,28 @@ int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_hea
  * every request stay visible).  Softmax over scale * q.k_j, plus the logit sinks[h] without a value row when sinks is
  * not null.  q bf16 [tokens][n_heads][head_dim], out bf16 [tokens][n_heads][v_head_dim]; (head_dim, v_head_dim) in
  * {(192,128), (128,128), (64,64)}; n_heads / n_kv_heads <= 128.  Cache slots that no query of the call sees may hold
- * anything, NaN included, and table entries of such pages are not read.  A request whose lengths do not fit (more
- * rows than positions, more positions than its table row, rows outside `tokens`) sets MIMO_ERANGE and gets no
- * output; a page outside the pool sets it too and reads as zeros. */
+ * anything, NaN included, and table entries of such pages are not read; what one query of a request sees must be finite
+ * in v, also for the queries before it.
+ *
+ * It takes two calls.  The plan deals the step's work to the SMs from its lengths; it holds for all layers with the
+ * same heads, window and keep_first (a caller-owned buffer, 16-byte aligned, of ..._plan_bytes).  A request whose
+ * lengths do not fit (more rows than positions, more positions than its table row, rows outside `tokens`) sets
+ * MIMO_ERANGE and gets no output.  The attention must be given the arguments that its plan was made with (otherwise
+ * status becomes MIMO_ERANGE and nothing is computed) on the same GPU; a page outside the pool sets MIMO_ERANGE and
+ * reads as zeros.  workspace: ..._workspace_bytes, 16-byte aligned, for one call at a time. */
+size_t mimo_moe_paged_attention_plan_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads);
+int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, int32_t R, int32_t tokens,
+                                  int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,
+                                  int32_t table_width, int32_t page_size, void* plan, size_t plan_bytes,
+                                  int32_t* status, void* stream);
+size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                                                int32_t v_head_dim);
 int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
-                             const int32_t* block_table, int32_t table_width, const int32_t* cu_q,
-                             const int32_t* seq_lens, int32_t R, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
-                             int32_t head_dim, int32_t v_head_dim, float scale, int32_t window, int32_t keep_first,
-                             int32_t num_pages, int32_t page_size, uint16_t* out, int32_t* status, void* stream);
+                             const int32_t* block_table, int32_t table_width, int32_t R, int32_t tokens,
+                             int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t v_head_dim, float scale,
+                             int32_t window, int32_t keep_first, int32_t num_pages, int32_t page_size,
+                             const void* plan, size_t plan_bytes, uint16_t* out, void* workspace,
+                             size_t workspace_bytes, int32_t* status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1204,23 +1204,78 @@ int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_hea
   return MIMO_OK;
 }
 
-int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
-                             const int32_t* block_table, int32_t table_width, const int32_t* cu_q,
-                             const int32_t* seq_lens, int32_t R, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
-                             int32_t head_dim, int32_t v_head_dim, float scale, int32_t window, int32_t keep_first,
-                             int32_t num_pages, int32_t page_size, uint16_t* out, int32_t* status, void* stream) {
-  if (!q || !k_pages || !v_pages || !block_table || !cu_q || !seq_lens || !out || tokens < 1 || n_heads < 1 ||
-      n_kv_heads < 1 || n_heads % n_kv_heads || n_heads / n_kv_heads > 128 ||
-      !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 || keep_first < 0 ||
-      (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) || bad_table(R, table_width, page_size) ||
-      !a16(q) || !a16(k_pages) || !a16(v_pages) || !a16(out))
+namespace {
+bool bad_heads(int32_t n_heads, int32_t n_kv_heads) {
+  return n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || n_heads / n_kv_heads > 128;
+}
+// What a plan depends on besides the lengths themselves, in one word (0 is no plan's).
+int32_t attn_plan_key(int32_t T, int32_t R, int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep,
+                      int32_t width, int32_t page_size, int32_t sms) {
+  uint32_t h = 2166136261u;
+  for (const int32_t v : {T, R, n_heads, n_kv_heads, window, keep, width, page_size, sms})
+    h = (h ^ (uint32_t)v) * 16777619u, h ^= h >> 15;
+  return (int32_t)(h | 1u);
+}
+}  // namespace
+
+size_t mimo_moe_paged_attention_plan_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads) {
+  if (tokens < 1 || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads)) return 0;
+  return attn_plan_bytes(tokens, R, n_heads / n_kv_heads, n_kv_heads, num_sms_current());
+}
+
+int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, int32_t R, int32_t tokens,
+                                  int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,
+                                  int32_t table_width, int32_t page_size, void* plan, size_t plan_bytes,
+                                  int32_t* status, void* stream) {
+  if (!cu_q || !seq_lens || !plan || tokens < 1 || bad_heads(n_heads, n_kv_heads) || window < 0 || keep_first < 0 ||
+      (keep_first > 0 && window == 0) || page_shift_of(page_size) < 0 || bad_table(R, table_width, page_size) ||
+      !a16(plan) || plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads))
     return MIMO_EINVAL;
-  PagedAttnParams p{};
-  p.q = q, p.k = k_pages, p.v = v_pages, p.sinks = sinks, p.table = block_table, p.cu_q = cu_q, p.seq_lens = seq_lens;
-  p.out = out, p.status = status, p.T = tokens, p.R = R, p.width = table_width, p.nq = n_heads, p.nkv = n_kv_heads;
+  AttnPlanParams p{};
+  const int sms = num_sms_current();
+  p.cu_q = cu_q, p.seq_lens = seq_lens, p.plan = static_cast<int32_t*>(plan), p.status = status;
+  p.T = tokens, p.R = R, p.G = n_heads / n_kv_heads, p.nkv = n_kv_heads, p.n = sms, p.width = table_width;
+  p.page_shift = page_shift_of(page_size), p.window = window, p.keep = keep_first;
+  p.merge_cost = 1 + paged_attn_part_rows(tokens, p.G) / 64;
+  p.key = attn_plan_key(tokens, R, n_heads, n_kv_heads, window, keep_first, table_width, page_size, sms);
+  MIMO_TRY(launch_attn_plan(p, static_cast<cudaStream_t>(stream)));
+  return MIMO_OK;
+}
+
+size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                                                int32_t v_head_dim) {
+  if (tokens < 1 || bad_heads(n_heads, n_kv_heads) || v_head_dim < 1) return 0;
+  return (size_t)2 * num_sms_current() * paged_attn_part_rows(tokens, n_heads / n_kv_heads) *
+         ((size_t)v_head_dim + 2) * 4;
+}
+
+int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
+                             const int32_t* block_table, int32_t table_width, int32_t R, int32_t tokens,
+                             int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t v_head_dim, float scale,
+                             int32_t window, int32_t keep_first, int32_t num_pages, int32_t page_size,
+                             const void* plan, size_t plan_bytes, uint16_t* out, void* workspace,
+                             size_t workspace_bytes, int32_t* status, void* stream) {
+  if (!q || !k_pages || !v_pages || !block_table || !plan || !out || !workspace || tokens < 1 ||
+      bad_heads(n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
+      keep_first < 0 || (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) ||
+      (int64_t)num_pages * n_kv_heads >= INT32_MAX || bad_table(R, table_width, page_size) || !a16(q) ||
+      !a16(k_pages) || !a16(v_pages) || !a16(out) || !a16(plan) || !a16(workspace) ||
+      plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads) ||
+      workspace_bytes < mimo_moe_paged_attention_workspace_bytes(tokens, n_heads, n_kv_heads, v_head_dim))
+    return MIMO_EINVAL;
+  PagedAttnParams p;
+  std::memset(&p, 0, sizeof(p));
+  const int sms = num_sms_current();
+  p.q = q, p.k = k_pages, p.v = v_pages, p.sinks = sinks, p.table = block_table;
+  p.plan = static_cast<const int32_t*>(plan), p.out = out, p.status = status;
+  p.T = tokens, p.R = R, p.width = table_width, p.nq = n_heads, p.nkv = n_kv_heads, p.G = n_heads / n_kv_heads;
   p.dqk = head_dim, p.dv = v_head_dim, p.window = window, p.keep = keep_first, p.num_pages = num_pages;
   p.page_shift = page_shift_of(page_size), p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  MIMO_TRY(launch_paged_attention(p, static_cast<cudaStream_t>(stream)));
+  p.part_rows = paged_attn_part_rows(tokens, p.G);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = p.part_o + (size_t)2 * sms * p.part_rows * v_head_dim;
+  p.key = attn_plan_key(tokens, R, n_heads, n_kv_heads, window, keep_first, table_width, page_size, sms);
+  MIMO_TRY(launch_paged_attention(p, sms, static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
 }
 

@@ -344,18 +344,31 @@ struct PagedRopeParams {
   float v_scale;    // already a bf16 value
   double log_base;  // ln(rope_theta)
 };
-struct PagedAttnParams {
-  const uint16_t *q, *k, *v;   // q [T][nq][dqk], pools [num_pages][nkv][page][d]
-  const float* sinks;          // [nq] sink logits, or null
-  const int32_t *table, *cu_q, *seq_lens;
-  uint16_t* out;               // [T][nq][dv]
-  int32_t* status;
-  int T, R, width, nq, nkv, dqk, dv, window, keep, num_pages, page_shift;
-  float scale_log2;            // softmax scale * log2(e)
+// The work plan of paged attention (paged_attn.cu): one of a step's lengths for each kind of layer.
+struct AttnPlanParams {
+  const int32_t *cu_q, *seq_lens;
+  int32_t *plan, *status;
+  int T, R, G, nkv, n, width, page_shift, window, keep;  // n: CTAs of the attention kernel
+  int merge_cost;                                        // of a split, in key blocks
+  int key;                                               // what the plan was made for
 };
+struct PagedAttnParams {
+  CUtensorMap qmap, kmap, vmap;  // q (box 64 dims x G heads x 128 / G tokens), pools (box 64 dims x a page)
+  const uint16_t *q, *k, *v;     // q [T][nq][dqk], pools [num_pages][nkv][page][d]
+  const float* sinks;            // [nq] sink logits, or null
+  const int32_t *table, *plan;
+  uint16_t* out;                 // [T][nq][dv]
+  float *part_o, *part_ml;       // [2 n][part_rows][dv] unnormalised parts, [2 n][part_rows][2] (max in log2, sum)
+  int32_t* status;
+  int T, R, width, nq, nkv, G, dqk, dv, window, keep, num_pages, page_shift, part_rows, key;
+  float scale_log2;              // softmax scale * log2(e)
+};
+size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms);
+int paged_attn_part_rows(int T, int G);  // query rows of the largest work unit
+cudaError_t launch_attn_plan(const AttnPlanParams& p, cudaStream_t st);
 cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st);
 cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st);
 cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st);
-cudaError_t launch_paged_attention(const PagedAttnParams& p, cudaStream_t st);
+cudaError_t launch_paged_attention(PagedAttnParams& p, int num_sms, cudaStream_t st);
 
 }  // namespace mimo

@@ -1,84 +1,844 @@
-// Attention of a step's new tokens over a paged KV cache (include/mimo_moe_paged.h).
+// Attention of a step's new tokens over a paged KV cache (include/mimo_moe_paged.h) on the 5th-generation tensor
+// cores: a plan of the step's work (one small launch, shared by all layers of a kind), the attention kernel (one
+// persistent CTA per SM) and the merge of what was split.
+//
+// A work unit is one kv head of up to 2 * (128 / G) consecutive new tokens of one request: two tiles A and B of 128
+// query rows (the G = n_heads / n_kv_heads heads of 128 / G tokens, token-major, so that one K/V block serves the whole
+// group and both tiles), over the blocks of 128 key positions that its queries see: blocks 0 .. nkb - 1 hold the first
+// tokens that stay visible, blocks lb .. the window (all, without one).
+//
+// One CTA, 12 warps:
+//   warps 0-3, 4-7   softmax of tile A and of tile B, one thread per query row (TMEM lane = row): the 128 scores of S_j
+//                    from TMEM into registers, mask, running maximum in the exp2 domain, P_j = bf16(2^(s - m)) back
+//                    over S_j's own TMEM columns, where the P V product reads it as its A operand (it never passes
+//                    through shared memory), the row sum from the float32 P.  The output in TMEM is rescaled only
+//                    when a row's maximum grows by more than 2^8 (P stays below 256);
+//   warp 8           TMA producer: Q of both tiles, then K_j and V_j as chunks of 64 dims x 128 positions (16 KB) through
+//                    one ring of shared-memory slots; lane i copies the i-th page of the block (a box of 64 dims x
+//                    page_size positions), and pages nobody sees are read as zeros from behind the pool's end;
+//   warp 9           MMA issuer (one thread): S = Q K^T and O += P V, alternating the tiles, so that one tile's products
+//                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV_j and
+//                    S_j+1 are issued in this order, so when S_j+1 is there, O holds PV_j and P_j is consumed;
+//   warp 10          zeroes the V rows that no query of the unit sees in the blocks at the range's ends: such slots may
+//                    hold anything, and 0 * NaN is not 0.
+// Every wait is bounded and sets MIMO_ETIMEOUT; the producer drains its copies and the issuer its MMAs before exit.
+#include <cstring>
+
 #include "common.cuh"
 #include "kernels.h"
+#include "tcgen05.cuh"
 
 namespace mimo {
 
 namespace {
 
-// One CTA per (token row, query head): four warps take the visible keys in turn, each with its own running maximum,
-// sum and output in float32; the four are joined at the end with the sink.
-template <int DQK, int DV>
-__global__ void __launch_bounds__(128) paged_attn_kernel(PagedAttnParams p) {
-  constexpr int QL = DQK / 32, VL = DV / 32;
-  __shared__ float sm_m[4], sm_l[4], sm_o[4][DV];
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kThreads = 384;
+// setmaxnreg: 2 x 128 softmax threads x 200 + 128 x 104 = 64512 = 384 x 168, what the block is launched with
+constexpr int kRegsSoftmax = 200, kRegsOther = 104;
+
+// ------------------------------------------------------------------------------------------------------------ the plan
+// Layout of the plan buffer (32-bit words, every part 16-byte aligned).
+struct PlanLayout {
+  int n, cap_tiles, cap_segs;
+  size_t base, count, merge, segs, tiles, nb, order, pre, words;
+};
+
+__host__ __device__ inline size_t up4(size_t x) { return (x + 3) & ~(size_t)3; }
+
+__host__ __device__ inline PlanLayout plan_layout(int T, int R, int G, int nkv, int n) {
+  PlanLayout L;
+  const int tok = 2 * (128 / G);
+  L.n = n;
+  L.cap_tiles = R + T / tok;  // sum of ceil(n_r / tok)
+  L.cap_segs = L.cap_tiles * nkv + n;
+  size_t at = 16;  // header: key, units, mode
+  L.base = at, at += up4(n);
+  L.count = at, at += up4(n);
+  L.merge = at, at += (size_t)8 * n;
+  L.segs = at, at += (size_t)8 * L.cap_segs;
+  L.tiles = at, at += (size_t)4 * L.cap_tiles;
+  L.nb = at, at += up4(L.cap_tiles);
+  L.order = at, at += up4(L.cap_tiles);
+  L.pre = at, at += up4((size_t)2 * L.cap_tiles + 2);
+  L.words = at;
+  return L;
+}
+
+// Key blocks of a unit whose queries are at qfirst .. qlast.
+struct Blocks {
+  int lo, keep, nkb, lb, n;
+};
+__device__ __forceinline__ Blocks blocks_of(int qfirst, int qlast, int window, int keep) {
+  Blocks b;
+  b.lo = window > 0 ? max(0, qfirst - window + 1) : 0;
+  b.keep = min(keep, b.lo);
+  b.lb = b.lo >> 7;
+  b.nkb = min((b.keep + 127) >> 7, b.lb);
+  b.n = b.nkb + (qlast >> 7) - b.lb + 1;
+  return b;
+}
+
+constexpr int kPlanThreads = 1024;
+constexpr int kBuckets = 2048;
+
+__device__ __forceinline__ long long block_scan(long long v, long long* excl, long long* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long a = __shfl_up_sync(0xFFFFFFFFu, x, o);
+    if (lane >= o) x += a;
+  }
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  long long base = 0, tot = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    const long long s = sh[w];
+    if (w < warp) base += s;
+    tot += s;
+  }
+  *excl = base + x - v;
+  __syncthreads();
+  return tot;
+}
+
+// One CTA.  Two ways to deal the units to the n CTAs: whole units, longest first, in a snake (no partial results), or
+// the units' blocks one after another in n equal ranges (perfect balance; a unit cut by a range's end leaves partial
+// results that the merge kernel joins).  The one whose longest CTA takes less is taken, in units of a key block.
+__global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams p) {
+  extern __shared__ int sm[];
+  int* toff = sm;                       // [R + 1] tiles before request r
+  __shared__ int hist[kBuckets];
+  __shared__ int load[1024];
+  __shared__ long long sh[kPlanThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const int t = blockIdx.x, h = blockIdx.y, hk = h / (p.nq / p.nkv);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (p.cu_q[p.R] > p.T && threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
-  if (t >= p.cu_q[p.R]) return;
-  int lo = 0, hi = p.R - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (p.cu_q[mid] <= t) lo = mid; else hi = mid - 1;
+  const int tid = threadIdx.x, n = p.n;
+  const int tok = 2 * (128 / p.G);
+  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, n);
+  int4* tiles = reinterpret_cast<int4*>(p.plan + L.tiles);
+  int* nbs = p.plan + L.nb;
+  int* order = p.plan + L.order;
+  long long* pre = reinterpret_cast<long long*>(p.plan + L.pre);
+  int4* segs = reinterpret_cast<int4*>(p.plan + L.segs);
+  int4* merge = reinterpret_cast<int4*>(p.plan + L.merge);
+  for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
+  load[tid] = 0;
+  // ---- tiles of each request; one whose lengths do not fit has none
+  {
+    const int per = (p.R + kPlanThreads - 1) / kPlanThreads, r0 = min(tid * per, p.R), r1 = min(r0 + per, p.R);
+    bool bad = tid == 0 && (p.cu_q[0] != 0 || p.cu_q[p.R] > p.T);
+    auto count = [&](int r) -> int {
+      const int a = p.cu_q[r], e = p.cu_q[r + 1], len = p.seq_lens[r];
+      if (a < 0 || e < a || e > p.T || len < e - a || (long long)len > ((long long)p.width << p.page_shift)) {
+        bad = true;
+        return 0;
+      }
+      return (e - a + tok - 1) / tok;
+    };
+    // the rows of all requests together are at most T, so the tiles fit cap_tiles; a table of overlapping rows could
+    // claim more, and is cut off there
+    long long mine = 0, ex;
+    for (int r = r0; r < r1; ++r) mine += count(r);
+    const long long tot = block_scan(mine, &ex, sh);
+    bad |= tot > L.cap_tiles;
+    for (int r = r0; r < r1; ++r) {
+      toff[r] = (int)min(ex, (long long)L.cap_tiles);
+      ex += count(r);
+    }
+    if (tid == 0) toff[p.R] = (int)min(tot, (long long)L.cap_tiles);
+    if (bad) set_status(p.status, MIMO_ERANGE);
   }
-  const int r = lo, row0 = p.cu_q[r], n = p.cu_q[r + 1] - row0, len = p.seq_lens[r];
-  if (row0 < 0 || n < 1 || t < row0 || t >= row0 + n || len < n || row0 + n > p.T ||
-      (long long)len > ((long long)p.width << p.page_shift)) {
-    if (threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
-    return;
-  }
-  const int pos = len - n + (t - row0);
-  const int first = p.window > 0 ? max(0, pos - p.window + 1) : 0;
-  const int keep = min(p.keep, first), seen = keep + pos - first + 1;
-  float q[QL], o[VL];
-#pragma unroll
-  for (int i = 0; i < QL; ++i) q[i] = bf16_to_f32(p.q[((size_t)t * p.nq + h) * DQK + lane + 32 * i]) * p.scale_log2;
-#pragma unroll
-  for (int i = 0; i < VL; ++i) o[i] = 0.f;
-  float m = -INFINITY, l = 0.f;
-  for (int s = warp; s < seen; s += 4) {
-    const int j = s < keep ? s : first + (s - keep);
-    const int page = p.table[(size_t)r * p.width + (j >> p.page_shift)];
-    const bool ok = (unsigned)page < (unsigned)p.num_pages;
-    if (!ok && lane == 0) set_status(p.status, MIMO_ERANGE);
-    const size_t at = (((size_t)(ok ? page : 0) * p.nkv + hk) << p.page_shift) + (j & ((1 << p.page_shift) - 1));
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < QL; ++i) dot = fmaf(q[i], ok ? bf16_to_f32(p.k[at * DQK + lane + 32 * i]) : 0.f, dot);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, x);
-    const float mn = fmaxf(m, dot), a = exp2f(m - mn), w = exp2f(dot - mn);
-    l = l * a + w;
-#pragma unroll
-    for (int i = 0; i < VL; ++i) o[i] = o[i] * a + w * (ok ? bf16_to_f32(p.v[at * DV + lane + 32 * i]) : 0.f);
-    m = mn;
-  }
-#pragma unroll
-  for (int i = 0; i < VL; ++i) sm_o[warp][lane + 32 * i] = o[i];
-  if (lane == 0) sm_m[warp] = m, sm_l[warp] = l;
   __syncthreads();
-  float M = p.sinks ? p.sinks[h] * 1.4426950408889634f : -INFINITY;
-  float L = 0.f;
-  const float sink = M;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
-  if (p.sinks) L = exp2f(sink - M);
-  for (int w = 0; w < 4; ++w) L += sm_l[w] * exp2f(sm_m[w] - M);
-  for (int d = threadIdx.x; d < DV; d += 128) {
-    float a = 0.f;
-    for (int w = 0; w < 4; ++w) a += sm_o[w][d] * exp2f(sm_m[w] - M);
-    p.out[((size_t)t * p.nq + h) * DV + d] = (uint16_t)f32_to_bf16(a / L);
+  const int nt = toff[p.R];
+  // ---- the tiles, their block counts and the prefix sums of these
+  long long W;
+  {
+    const int per = (nt + kPlanThreads - 1) / kPlanThreads, i0 = min(tid * per, nt), i1 = min(i0 + per, nt);
+    long long mine = 0, ex;
+    int r = 0;
+    if (i0 < i1) {
+      int lo = 0, hi = p.R - 1;  // the last request with toff <= i0 (requests without tiles share an offset)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (toff[mid] <= i0) lo = mid; else hi = mid - 1;
+      }
+      r = lo;
+    }
+    for (int i = i0; i < i1; ++i) {
+      while (toff[r + 1] <= i) ++r;
+      const int a = p.cu_q[r], rows = p.cu_q[r + 1] - a, t0 = (i - toff[r]) * tok;
+      const int ntok = min(tok, rows - t0), qfirst = p.seq_lens[r] - rows + t0;
+      const int nb = blocks_of(qfirst, qfirst + ntok - 1, p.window, p.keep).n;
+      tiles[i] = make_int4(a + t0, ntok, qfirst, r);
+      nbs[i] = nb;
+      atomicAdd(&hist[kBuckets - 1 - min(nb, kBuckets - 1)], 1);
+      mine += nb;
+    }
+    W = block_scan(mine, &ex, sh);
+    for (int i = i0; i < i1; ++i) {
+      pre[i] = ex;
+      ex += nbs[i];
+    }
+    if (tid == 0) pre[nt] = W;
   }
+  // ---- longest first
+  {
+    constexpr int per = kBuckets / kPlanThreads;
+    long long mine = 0, ex;
+    int c[per];
+#pragma unroll
+    for (int k = 0; k < per; ++k) c[k] = hist[tid * per + k], mine += c[k];
+    block_scan(mine, &ex, sh);
+#pragma unroll
+    for (int k = 0; k < per; ++k) {
+      hist[tid * per + k] = (int)ex;
+      ex += c[k];
+    }
+    __syncthreads();
+    for (int i = tid; i < nt; i += kPlanThreads)
+      order[atomicAdd(&hist[kBuckets - 1 - min(nbs[i], kBuckets - 1)], 1)] = i;
+    __syncthreads();
+  }
+  const int units = nt * p.nkv;
+  W *= p.nkv;
+  const int K = (units + n - 1) / n;  // rounds of the snake
+  auto cta_of = [&](int u) -> int {
+    const int k = u / n, c = u % n;
+    return (k & 1) ? n - 1 - c : c;
+  };
+  for (int u = tid; u < units; u += kPlanThreads) atomicAdd(&load[cta_of(u)], nbs[order[u / p.nkv]] + 1);
+  __syncthreads();
+  int most = tid < n ? load[tid] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, o));
+  __syncthreads();
+  if ((tid & 31) == 0) load[tid >> 5] = most;
+  __syncthreads();
+  for (int w = 0; w < kPlanThreads / 32; ++w) most = max(most, load[w]);
+  // a CTA's range holds at least two blocks: a shorter one costs more in its partial result than it saves
+  const long long quota = max(2ll, (W + n - 1) / n);
+  const bool split = quota + (units + n - 1) / n + p.merge_cost < most;
+  if (tid == 0) {
+    p.plan[1] = units;
+    p.plan[2] = split ? 1 : 0;
+    p.plan[0] = p.key;
+  }
+  int* base = p.plan + L.base;
+  int* cnt = p.plan + L.count;
+  for (int c = tid; c < n; c += kPlanThreads) {
+    merge[2 * c] = make_int4(0, 0, 0, 0);
+    if (!split) {
+      const int full = units / n, rest = units % n;
+      base[c] = c * K;
+      cnt[c] = full + (((full & 1) ? n - 1 - c : c) < rest ? 1 : 0);
+    } else if (c * quota >= W) {
+      base[c] = 0, cnt[c] = 0;
+    } else {
+      // the unit that holds block x of the line of all units' blocks
+      auto unit_at = [&](long long x) -> int {
+        int lo = 0, hi = nt - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (pre[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
+        }
+        return lo * p.nkv + (int)((x - pre[lo] * p.nkv) / nbs[lo]);
+      };
+      const int first = unit_at(c * quota), last = unit_at(min(W, (c + 1) * quota) - 1);
+      base[c] = first + c;
+      cnt[c] = last - first + 1;
+    }
+  }
+  __syncthreads();
+  for (int u = tid; u < units; u += kPlanThreads) {
+    if (!split) {
+      const int i = order[u / p.nkv], c = cta_of(u);
+      int4* s = segs + 2 * ((size_t)c * K + u / n);
+      s[0] = tiles[i];
+      s[1] = make_int4(u % p.nkv, 0, nbs[i], -1);
+    } else {
+      const int i = u / p.nkv, hk = u % p.nkv, nb = nbs[i];
+      const int4 t = tiles[i];
+      const long long s0 = pre[i] * p.nkv + (long long)hk * nb, s1 = s0 + nb;
+      const int c0 = (int)(s0 / quota), c1 = (int)((s1 - 1) / quota);
+      int slot0 = -1;
+      for (int c = c0; c <= c1; ++c) {
+        const int b0 = (int)(max(s0, c * quota) - s0), b1 = (int)(min(s1, (c + 1) * quota) - s0);
+        const int slot = c0 == c1 ? -1 : 2 * c + (base[c] == u + c ? 0 : 1);  // a CTA's first segment, or its last
+        if (c == c0) slot0 = slot;
+        int4* s = segs + 2 * ((size_t)u + c);
+        s[0] = t;
+        s[1] = make_int4(hk, b0, b1 - b0, slot);
+      }
+      if (c1 > c0) {  // at most one unit runs over the end of CTA c0's range
+        merge[2 * c0] = make_int4(t.x, t.y, hk, c0);
+        merge[2 * c0 + 1] = make_int4(slot0, c1 - c0 + 1, 0, 0);
+      }
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------- attention
+__device__ __forceinline__ float ex2_approx(float x) {  // 2^x on the special-function unit: 2^-inf = +0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2_rn(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 32 TMEM columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// MN-major operand, 128B swizzle: 64 contiguous values (128 B) along N per row of K, 8 rows per 1024-byte atom; LBO =
+// stride between groups of 64 values along N, SBO = stride between groups of 8 rows along K.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
+         (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// kind::f16 with A in TMEM: lane = row of A, a 32-bit column holds two consecutive values along K.
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+
+constexpr uint32_t kChunk = 16384;  // 128 positions x 64 dims, bf16
+
+template <int DQK, int DV>
+struct Shape {
+  static constexpr int QCH = DQK / 64, VCH = DV / 64;
+  static constexpr uint32_t QB = 128u * DQK * 2;
+  static constexpr int NS = (int)((232448u - 2048u - 2 * QB) / kChunk);  // ring slots in what Q leaves
+  static constexpr uint32_t SMEM = 2048 + 2 * QB + NS * kChunk;          // barriers, alignment slack, tiles
+};
+
+struct Seg {
+  int row0, ntok, qfirst, r, hk, b0, nblk, slot;
+};
+
+template <int DQK, int DV>
+__global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+  using S = Shape<DQK, DV>;
+  constexpr int NS = S::NS, CPB = S::QCH + S::VCH;  // ring slots, chunks per block
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* full = bars;
+  uint64_t* empty = full + NS;
+  uint64_t* q_full = empty + NS;
+  uint64_t* q_empty = q_full + 2;
+  uint64_t* s_full = q_empty + 2;
+  uint64_t* p_full = s_full + 2;
+  uint64_t* o_full = p_full + 2;
+  uint64_t* fix_req = o_full + 2;
+  uint64_t* v_fixed = fix_req + 1;
+  uint64_t* drain = v_fixed + 1;
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)(smem + 1024) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = base;
+  uint8_t* sRing = base + 2 * S::QB;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+    }
+    mbar_init(fix_req, 1);
+    mbar_init(v_fixed, 1);
+    mbar_init(drain, 1);
+    mbar_fence_init();
+  }
+  if (warp == 9) {
+    tc::tmem_alloc(tslot, 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tbase = *tslot;
+  pdl_wait();  // q, the cache and the plan come from preceding kernels (programmatic dependent launch)
+  pdl_launch_dependents();
+
+  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, gridDim.x);
+  const bool planned = p.plan[0] == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
+  if (!planned && threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
+  const int sbase = planned ? p.plan[L.base + blockIdx.x] : 0, nseg = planned ? p.plan[L.count + blockIdx.x] : 0;
+  const int4* segs = reinterpret_cast<const int4*>(p.plan + L.segs) + 2 * (size_t)sbase;
+  const int tpt = 128 / p.G;  // tokens per tile
+  auto load_seg = [&](int s) -> Seg {
+    const int4 a = segs[2 * s], b = segs[2 * s + 1];
+    return Seg{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  };
+  bool ok = true;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
+    if (warp == 8) {  // ------------------------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        tma_prefetch_map(&p.qmap);
+        tma_prefetch_map(&p.kmap);
+        tma_prefetch_map(&p.vmap);
+      }
+      const uint64_t pol = tc::l2_evict_normal_policy();
+      const int P = 1 << p.page_shift, ppb = 128 >> p.page_shift;  // pages per block
+      const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
+      uint32_t ci = 0;                                             // chunks issued
+      uint32_t nq[2] = {0, 0};                                     // Q loads of each tile
+      for (int s = 0; s < nseg && ok; ++s) {
+        const Seg g = load_seg(s);
+        const int qlast = g.qfirst + g.ntok - 1;
+        const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
+        const int* trow = p.table + (size_t)g.r * p.width;
+        // the page (its row in the maps) that this lane copies of block j
+        auto page_of = [&](int j) -> int {
+          const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb);
+          const int pg = kb * ppb + lane, pos = pg << p.page_shift;
+          if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return nowhere;
+          const int id = trow[pg];
+          if ((unsigned)id >= (unsigned)p.num_pages) {
+            set_status(p.status, MIMO_ERANGE);
+            return nowhere;
+          }
+          return id * p.nkv + g.hk;
+        };
+        int row = page_of(g.b0);
+        for (int j = 0; j < g.nblk && ok; ++j) {
+          const int next = j + 1 < g.nblk ? page_of(g.b0 + j + 1) : 0;
+#pragma unroll
+          for (int c = 0; c < CPB; ++c) {
+            if (c == S::QCH && j == 0) {  // Q behind the first K block
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                if (x == 1 && g.ntok <= tpt) break;
+                if (ok) ok = mbar_wait(&q_empty[x], (nq[x] & 1) ^ 1);
+                ++nq[x];
+                if (lane == 0 && ok) {
+                  mbar_arrive_expect_tx(&q_full[x], (uint32_t)(S::QCH * 128 * p.G * tpt));
+#pragma unroll
+                  for (int d = 0; d < S::QCH; ++d)
+                    tma_load_3d(sQ + x * S::QB + d * kChunk, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[x],
+                                pol);
+                }
+              }
+            }
+            const uint32_t sl = ci % NS;
+            if (ok) ok = mbar_wait(&empty[sl], ((ci / NS) & 1) ^ 1);
+            ok = __all_sync(0xFFFFFFFFu, ok);
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&full[sl], kChunk);
+            __syncwarp();
+            if (lane < ppb) {
+              uint8_t* dst = sRing + sl * kChunk + (uint32_t)lane * P * 128;
+              if (c < S::QCH)
+                tma_load_3d(dst, &p.kmap, c * 64, 0, row, &full[sl], pol);
+              else
+                tma_load_3d(dst, &p.vmap, (c - S::QCH) * 64, 0, row, &full[sl], pol);
+            }
+            ++ci;
+          }
+          row = next;
+        }
+      }
+      // no copy may still be landing when the CTA exits: the last chunk of every slot, and Q
+      for (uint32_t k = 0; k < (uint32_t)NS && k < ci; ++k) {
+        const uint32_t i = ci - 1 - k;
+        mbar_wait(&full[i % NS], (i / NS) & 1);
+      }
+      for (int x = 0; x < 2; ++x)
+        if (nq[x]) mbar_wait(&q_full[x], (nq[x] - 1) & 1);
+    } else if (warp == 9) {
+      if (lane == 0) {  // ------------------------------------------------------------------------- MMA issuer
+        const uint32_t idesc_s = tc::idesc_bf16(128, 128);
+        const uint32_t idesc_o64 = tc::idesc_bf16(128, 64) | (1u << 16);  // B = V, MN-major
+        const uint32_t idesc_o = tc::idesc_bf16(128, DV) | (1u << 16);
+        const uint32_t aq = smem_u32(sQ), ar = smem_u32(sRing);
+        uint32_t ci = 0;  // chunks of the blocks before this one
+        uint32_t ns[2] = {0, 0}, np[2] = {0, 0}, fixes = 0;
+        auto chunks_there = [&](uint32_t at, int n) {
+          for (int c = 0; c < n && ok; ++c) ok = mbar_wait(&full[(at + c) % NS], ((at + c) / NS) & 1);
+          tc::tc_fence_after();
+        };
+        // S = Q K^T of tile x from the K chunks at ring position `at`; the last tile to read them frees each
+        auto issue_s = [&](int x, uint32_t at, bool frees) {
+#pragma unroll
+          for (int c = 0; c < S::QCH; ++c) {
+            const uint32_t sl = (at + c) % NS;
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              tc::tc_mma_f16(tbase + x * 128, tc::desc_sw128(aq + x * S::QB + c * kChunk + kk * 32),
+                             tc::desc_sw128(ar + sl * kChunk + kk * 32), idesc_s, (c | kk) != 0 ? 1u : 0u);
+            if (frees) tc::tc_commit(&empty[sl]);
+          }
+          tc::tc_commit(&s_full[x]);
+        };
+        auto issue_pv = [&](int x, uint32_t at, bool first, bool frees) {
+          const uint32_t d = tbase + 256 + x * DV, a = tbase + x * 128;
+          const uint32_t sl = at % NS;
+          if (S::VCH == 2 && sl + 1 < (uint32_t)NS) {  // the two V chunks lie one behind the other
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk)
+              tc_mma_f16_ts(d, a + kk * 8, desc_mn_sw128(ar + sl * kChunk + kk * 2048, kChunk, 1024), idesc_o,
+                            (!first || kk != 0) ? 1u : 0u);
+          } else {
+#pragma unroll
+            for (int c = 0; c < S::VCH; ++c)
+#pragma unroll
+              for (int kk = 0; kk < 8; ++kk)
+                tc_mma_f16_ts(d + c * 64, a + kk * 8,
+                              desc_mn_sw128(ar + ((at + c) % NS) * kChunk + kk * 2048, kChunk, 1024), idesc_o64,
+                              (!first || kk != 0) ? 1u : 0u);
+          }
+          if (frees)
+            for (int c = 0; c < S::VCH; ++c) tc::tc_commit(&empty[(at + c) % NS]);
+        };
+        for (int s = 0; s < nseg && ok; ++s) {
+          const Seg g = load_seg(s);
+          const int qlast = g.qfirst + g.ntok - 1;
+          const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
+          const int nx = g.ntok > tpt ? 2 : 1;
+          chunks_there(ci, S::QCH);
+          for (int x = 0; x < nx && ok; ++x) {
+            ok = mbar_wait(&q_full[x], ns[x] & 1);
+            ++ns[x];
+            tc::tc_fence_after();
+            if (!ok) break;
+            issue_s(x, ci, x == nx - 1);
+            if (g.nblk == 1) tc::tc_commit(&q_empty[x]);
+          }
+          for (int j = 0; j < g.nblk && ok; ++j) {
+            const int kb = g.b0 + j < bl.nkb ? g.b0 + j : bl.lb + (g.b0 + j - bl.nkb);
+            const int kp = kb * 128;
+            const uint32_t at = ci + S::QCH;
+            // some rows of V are nobody's: zeroed while the softmax runs
+            const bool fix = !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
+            chunks_there(at, S::VCH);
+            if (fix && ok) mbar_arrive(fix_req);
+            const bool more = j + 1 < g.nblk;
+            for (int x = 0; x < nx && ok; ++x) {
+              ok = mbar_wait(&p_full[x], np[x] & 1);
+              ++np[x];
+              if (x == 0 && fix && ok) ok = mbar_wait(v_fixed, fixes++ & 1);
+              tc::tc_fence_after();
+              if (!ok) break;
+              issue_pv(x, at, j == 0, x == nx - 1);
+              if (more) {
+                if (x == 0) chunks_there(ci + CPB, S::QCH);
+                if (!ok) break;
+                issue_s(x, ci + CPB, x == nx - 1);
+                if (j + 2 == g.nblk) tc::tc_commit(&q_empty[x]);
+              } else {
+                tc::tc_commit(&o_full[x]);
+              }
+            }
+            ci += CPB;
+          }
+        }
+        tc::tc_commit(drain);  // every MMA issued above has completed once this arrives
+        if (!mbar_wait(drain, 0)) ok = false;
+      }
+    } else if (warp == 10) {  // --------------------------------------------------- zeroes what nobody sees of V
+      uint32_t ci = 0, fixes = 0;
+      for (int s = 0; s < nseg && ok; ++s) {
+        const Seg g = load_seg(s);
+        const int qlast = g.qfirst + g.ntok - 1;
+        const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
+        for (int j = 0; j < g.nblk && ok; ++j, ci += CPB) {
+          const int kb = g.b0 + j < bl.nkb ? g.b0 + j : bl.lb + (g.b0 + j - bl.nkb);
+          const int kp = kb * 128;
+          if (kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep)) continue;
+          ok = mbar_wait(fix_req, fixes++ & 1);  // the block's V is there
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < S::VCH; ++c) {
+            uint8_t* chunk = sRing + ((ci + S::QCH + c) % NS) * kChunk;
+            // a row is 128 bytes whatever the swizzle: 8 lanes a row
+            for (int row = lane >> 3; row < 128; row += 4) {
+              const int pos = kp + row;
+              if (pos > qlast || (pos < bl.lo && pos >= bl.keep))
+                *reinterpret_cast<uint4*>(chunk + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          tc::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(v_fixed);
+        }
+      }
+    }
+  } else {  // ------------------------------------------------------------------------------- softmax of tile x
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
+    const int x = warp >> 2, r = threadIdx.x & 127;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t tS = tbase + x * 128 + lane_off, tO = tbase + 256 + x * DV + lane_off;
+    const int tt = r / p.G + x * tpt, head = r % p.G;  // this row's token of the unit and head of the group
+    const float sl2 = p.scale_log2;
+    uint32_t ns = 0, no = 0;
+    for (int s = 0; s < nseg && ok; ++s) {
+      const Seg g = load_seg(s);
+      if (x == 1 && g.ntok <= tpt) continue;
+      const Blocks bl = blocks_of(g.qfirst, g.qfirst + g.ntok - 1, p.window, p.keep);
+      const bool row_ok = r < tpt * p.G && tt < g.ntok;
+      const bool work = __any_sync(0xFFFFFFFFu, row_ok);  // a warp without a row only keeps the barriers going
+      const int qpos = row_ok ? g.qfirst + tt : -1;
+      const int lo = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
+      const int keep = min(p.keep, lo);
+      float m_ref = -INFINITY, l = 0.f;
+      for (int j = 0; j < g.nblk; ++j) {
+        if (ok) ok = mbar_wait(&s_full[x], ns & 1);
+        ++ns;
+        ok = __all_sync(0xFFFFFFFFu, ok);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (work) {
+          float v[128];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, v + c * 32);
+          tc::tmem_wait_ld();
+          const int jb = g.b0 + j, kp = (jb < bl.nkb ? jb : bl.lb + (jb - bl.nkb)) * 128;
+          if (!(kp + 127 <= qpos && (kp >= lo || kp + 127 < keep))) {
+            const int c_hi = qpos - kp, c_lo = lo - kp, c_keep = keep - kp;
+#pragma unroll
+            for (int c = 0; c < 128; ++c)
+              if (c > c_hi || (c < c_lo && c >= c_keep)) v[c] = -INFINITY;
+          }
+          float mx[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float a = v[c * 32];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) a = fmaxf(a, v[c * 32 + e]);
+            mx[c] = a;
+          }
+          // the scale is positive, so it orders the scaled scores alike
+          const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
+          float alpha = 1.f;
+          bool rescale = false;
+          if (m > -INFINITY) {
+            if (m_ref == -INFINITY) {
+              m_ref = m;
+            } else if (m > m_ref + 8.f) {
+              alpha = ex2_approx(m_ref - m);
+              m_ref = m;
+              rescale = true;
+            }
+          }
+          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
+          float sum[4] = {0.f, 0.f, 0.f, 0.f};
+          uint32_t pk[64];
+#pragma unroll
+          for (int i = 0; i < 64; ++i) {
+            const float p0 = ex2_approx(fmaf(v[2 * i], sl2, nm)), p1 = ex2_approx(fmaf(v[2 * i + 1], sl2, nm));
+            sum[i & 3] += p0 + p1;
+            pk[i] = pack_bf16x2_rn(p0, p1);  // P is rounded to bf16 for the product with V, the sum is not
+          }
+          l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+          if (__any_sync(0xFFFFFFFFu, rescale)) {  // O holds the product of the block before (see above)
+#pragma unroll 1
+            for (int c = 0; c < DV; c += 32) {
+              float o[32];
+              tmem_ld32(tO + c, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] *= alpha;
+              tmem_st32(tO + c, reinterpret_cast<const uint32_t*>(o));
+            }
+          }
+          tmem_st32(tS, pk);
+          tmem_st32(tS + 32, pk + 32);
+          tmem_wait_st();
+        }
+        tc::tc_fence_before();
+        mbar_arrive(&p_full[x]);
+      }
+      if (ok) ok = mbar_wait(&o_full[x], no & 1);
+      ++no;
+      ok = __all_sync(0xFFFFFFFFu, ok);
+      if (!ok) break;
+      tc::tc_fence_after();
+      if (!work) continue;
+      const int qh = g.hk * p.G + head, row = g.row0 + tt;
+      if (g.slot < 0) {
+        float f;
+        if (p.sinks) {
+          const float sk = (row_ok ? p.sinks[qh] : 0.f) * kLog2e;
+          const float M = fmaxf(m_ref, sk);
+          const float a = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
+          f = a / (l * a + exp2f(sk - M));
+        } else {
+          f = l > 0.f ? 1.f / l : 0.f;
+        }
+        uint16_t* dst = p.out + ((size_t)row * p.nq + qh) * DV;
+#pragma unroll 1
+        for (int c = 0; c < DV; c += 32) {
+          float o[32];
+          tmem_ld32(tO + c, o);
+          tc::tmem_wait_ld();
+          if (row_ok && row < p.T) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2_rn(o[e * 8 + 2 * k] * f, o[e * 8 + 2 * k + 1] * f);
+              reinterpret_cast<uint4*>(dst + c)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      } else {  // an unnormalised part: maximum (log2), sum and output of these blocks
+        const size_t at = (size_t)g.slot * p.part_rows + (tt * p.G + head);
+#pragma unroll 1
+        for (int c = 0; c < DV; c += 32) {
+          float o[32];
+          tmem_ld32(tO + c, o);
+          tc::tmem_wait_ld();
+          if (row_ok) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + at * DV + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (row_ok) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
+      }
+      tc::tc_fence_before();
+    }
+  }
+  if (!ok && p.status) set_status(p.status, MIMO_ETIMEOUT);
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tbase, 512);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ merge
+// Joins the parts of the unit that runs over the end of CTA blockIdx.x's range: a warp per query row, in the order of
+// the parts, so that the result does not depend on when they were done.
+constexpr int kMergeWarps = 8;
+
+template <int DV>
+__global__ void __launch_bounds__(kMergeWarps * 32) paged_attn_merge_kernel(const __grid_constant__ PagedAttnParams p) {
+  constexpr int VL = DV / 32;
+  pdl_wait();
+  pdl_launch_dependents();
+  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, gridDim.x);
+  if (p.plan[0] != p.key) return;
+  const int4* mg = reinterpret_cast<const int4*>(p.plan + L.merge) + 2 * (size_t)blockIdx.x;
+  const int4 a = mg[0], b = mg[1];  // row0, tokens, kv head, first CTA; slot of the first part, parts
+  const int lane = threadIdx.x & 31;
+  for (int rr = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); rr < a.y * p.G; rr += gridDim.y * kMergeWarps) {
+    const int tt = rr / p.G, qh = a.z * p.G + rr % p.G, row = a.x + tt;
+    auto part = [&](int s) -> size_t { return (size_t)(s == 0 ? b.x : 2 * (a.w + s)) * p.part_rows + rr; };
+    const float sink = p.sinks ? p.sinks[qh] * kLog2e : -INFINITY;
+    float M = sink;
+    for (int s = lane; s < b.y; s += 32) M = fmaxf(M, p.part_ml[part(s) * 2]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+    float sum = p.sinks ? exp2f(sink - M) : 0.f, acc[VL];
+#pragma unroll
+    for (int k = 0; k < VL; ++k) acc[k] = 0.f;
+    for (int s0 = 0; s0 < b.y; s0 += 32) {
+      float w = 0.f, wl = 0.f;
+      if (s0 + lane < b.y) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part(s0 + lane) * 2);
+        w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
+        wl = w * ml.y;
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) wl += __shfl_xor_sync(0xFFFFFFFFu, wl, o);
+      sum += wl;
+      const int e = min(32, b.y - s0);
+#pragma unroll 8
+      for (int s = 0; s < e; ++s) {
+        const float f = __shfl_sync(0xFFFFFFFFu, w, s);
+        const float2* src = reinterpret_cast<const float2*>(p.part_o + part(s0 + s) * DV + lane * VL);
+#pragma unroll
+        for (int k = 0; k < VL / 2; ++k) {
+          const float2 o = src[k];
+          acc[2 * k] = fmaf(f, o.x, acc[2 * k]);
+          acc[2 * k + 1] = fmaf(f, o.y, acc[2 * k + 1]);
+        }
+      }
+    }
+    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    if (row >= p.T) continue;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((size_t)row * p.nq + qh) * DV + lane * VL);
+#pragma unroll
+    for (int k = 0; k < VL / 2; ++k) dst[k] = pack_bf16x2_rn(acc[2 * k] * f, acc[2 * k + 1] * f);
+  }
+}
+
+template <int DQK, int DV>
+cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
+  using S = Shape<DQK, DV>;
+  static bool attr_set[128] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 128 && !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<DQK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)S::SMEM);
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  const cudaError_t e = launch_k(paged_attn_kernel<DQK, DV>, dim3(num_sms), dim3(kThreads), S::SMEM, st, p);
+  if (e != cudaSuccess) return e;
+  return launch_k(paged_attn_merge_kernel<DV>, dim3(num_sms, std::min(4, (p.part_rows + kMergeWarps - 1) / kMergeWarps)),
+                  dim3(kMergeWarps * 32), 0, st, p);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_attention(const PagedAttnParams& p, cudaStream_t st) {
-  const dim3 grid(p.T, p.nq);
-  if (p.dqk == 192) return launch_k(paged_attn_kernel<192, 128>, grid, dim3(128), 0, st, p);
-  if (p.dqk == 128) return launch_k(paged_attn_kernel<128, 128>, grid, dim3(128), 0, st, p);
-  return launch_k(paged_attn_kernel<64, 64>, grid, dim3(128), 0, st, p);
+size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms) {
+  return plan_layout(T, R, G, nkv, num_sms).words * 4;
+}
+
+int paged_attn_part_rows(int T, int G) { return std::min(2 * (128 / G), T) * G; }
+
+cudaError_t launch_attn_plan(const AttnPlanParams& p, cudaStream_t st) {
+  return launch_k(attn_plan_kernel, dim3(1), dim3(kPlanThreads), (size_t)(p.R + 1) * 4, st, p);
+}
+
+cudaError_t launch_paged_attention(PagedAttnParams& p, int num_sms, cudaStream_t st) {
+  const uint64_t rows = (uint64_t)p.num_pages * p.nkv;
+  const int P = 1 << p.page_shift;
+  cudaError_t e = bf16_map3(&p.qmap, p.q, (uint64_t)p.dqk, (uint64_t)p.nq, (uint64_t)p.T, p.G, 128 / p.G);
+  if (e == cudaSuccess) e = bf16_map3(&p.kmap, p.k, (uint64_t)p.dqk, (uint64_t)P, rows, P, 1);
+  if (e == cudaSuccess) e = bf16_map3(&p.vmap, p.v, (uint64_t)p.dv, (uint64_t)P, rows, P, 1);
+  if (e != cudaSuccess) return e;
+  if (p.dqk == 192) return launch_t<192, 128>(p, num_sms, st);
+  if (p.dqk == 128) return launch_t<128, 128>(p, num_sms, st);
+  return launch_t<64, 64>(p, num_sms, st);
 }
 
 }  // namespace mimo

@@ -223,7 +223,8 @@ class PageTable:
 
 class PagedKVCache:
     """Paged KV cache of one attention layer: k [num_pages, n_kv, page_size, head_dim], v [num_pages, n_kv, page_size,
-    v_head_dim] bf16 (new and zeroed, or the tensors given).  `step` is the PageStep the layer's next call works on."""
+    v_head_dim] bf16 (new and zeroed, or the tensors given).  `step` is the PageStep the layer's next call works on, `plan`
+    that step's attention plan for the layer's kind (None: made at the call)."""
 
     paged = True
 
@@ -241,6 +242,7 @@ class PagedKVCache:
         self.k, self.v = _buffer(k, "k", ks, k.device), _buffer(v, "v", vs, k.device)
         self.device = k.device
         self.step: Optional[PageStep] = None
+        self.plan: Optional["AttentionPlan"] = None
         self._out = {}
 
     def attend(self, qkv: torch.Tensor, sinks: Optional[torch.Tensor]) -> torch.Tensor:
@@ -253,7 +255,7 @@ class PagedKVCache:
         if shape not in self._out:
             self._out[shape] = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
         q = rope_store_paged(qkv, cfg, self, step)
-        return attention_paged(q, self, cfg, step, sinks, out=self._out[shape])
+        return attention_paged(q, self, cfg, step, sinks, plan=self.plan, out=self._out[shape])
 
 
 def _fits(cache: PagedKVCache, cfg: AttentionConfig, step: PageStep, where: str) -> None:
@@ -285,14 +287,44 @@ def rope_store_paged(qkv: torch.Tensor, cfg: AttentionConfig, cache: PagedKVCach
     return q
 
 
+def _kind(cfg: AttentionConfig):
+    """What layers of one attention plan have in common."""
+    return cfg.n_heads, cfg.n_kv_heads, cfg.window, cfg.keep_first
+
+
 class AttentionPlan:
-    """What attention_paged works out of a step's lengths for one kind of layer (one for all its layers)."""
+    """How attention_paged deals a step's work to the SMs, made from the step's lengths: one for all layers with the
+    same heads, window and keep_first (attention_plan).  It holds until the step's lengths change."""
 
     def __init__(self, step: PageStep, cfg: AttentionConfig):
-        self.step, self.cfg = step, cfg
+        if cfg.keep_first and not cfg.window:
+            raise ValueError("attention_plan: keep_first needs a window (without one every earlier token is visible)")
+        if cfg.n_heads < 1 or cfg.n_kv_heads < 1 or cfg.n_heads % cfg.n_kv_heads or cfg.n_heads // cfg.n_kv_heads > 128:
+            raise ValueError(f"attention_plan: {cfg.n_heads} heads over {cfg.n_kv_heads} kv heads")
+        self.step, self.kind = step, _kind(cfg)
+        self.buffer = None
+        if step.tokens == 0:
+            return
+        with _on(step.device):
+            L = lib()
+            nb = L.mimo_moe_paged_attention_plan_bytes(step.tokens, step.requests, cfg.n_heads, cfg.n_kv_heads)
+            self.buffer = torch.empty(nb, dtype=torch.uint8, device=step.device)
+            self.update()
+
+    def update(self) -> None:
+        """Make the plan again from the step's present lengths, in the same buffer."""
+        step, (nq, nkv, window, keep) = self.step, self.kind
+        if self.buffer is None:
+            return
+        with _on(step.device):
+            check(lib().mimo_moe_paged_attention_plan(step.cu_q.data_ptr(), step.seq_lens.data_ptr(), step.requests,
+                                                      step.tokens, nq, nkv, window, keep, step.width, step.page_size,
+                                                      self.buffer.data_ptr(), self.buffer.numel(),
+                                                      step.status.data_ptr(), _stream(step.device)), "attention_plan")
 
 
 def attention_plan(step: PageStep, cfg: AttentionConfig) -> AttentionPlan:
+    """The plan of a step for the layers of cfg's kind, for attention_paged(..., plan=)."""
     return AttentionPlan(step, cfg)
 
 
@@ -300,12 +332,11 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
                     sinks: Optional[torch.Tensor] = None, plan: Optional[AttentionPlan] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """mimo_moe.layer.attention for a step's token rows over the paged cache: causal; with cfg.window a sliding window,
-    in which each request's first cfg.keep_first tokens stay visible; sinks float32 [n_heads].  Returns bf16
-    [tokens, n_heads, v_head_dim]; padding rows of a given `out` are not written, those of a new one are zero."""
+    in which each request's first cfg.keep_first tokens stay visible; sinks float32 [n_heads].  plan: the step's
+    attention_plan for this kind of layer (made for this call when None).  Returns bf16 [tokens, n_heads, v_head_dim];
+    padding rows of a given `out` are not written, those of a new one are zero."""
     _fits(cache, cfg, step, "attention_paged")
     T, dev = step.tokens, step.device
-    if cfg.keep_first and not cfg.window:
-        raise ValueError("attention_paged: keep_first needs a window (without one every earlier token is visible)")
     q = _bf16(q, "q", (T, cfg.n_heads, cfg.head_dim), dev)
     shape = (T, cfg.n_heads, cfg.v_head_dim)
     o = torch.zeros(shape, dtype=torch.bfloat16, device=dev) if out is None else _buffer(out, "out", shape, dev)
@@ -313,15 +344,22 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
         if tuple(sinks.shape) != (cfg.n_heads,):
             raise ValueError(f"attention_paged: {cfg.n_heads} heads need as many sinks, got {tuple(sinks.shape)}")
         sinks = sinks.to(device=dev, dtype=torch.float32).contiguous()
+    if plan is None:
+        plan = AttentionPlan(step, cfg)
+    elif plan.step is not step or plan.kind != _kind(cfg):
+        raise ValueError("attention_paged: the plan was made for another step or kind of layer")
     if T == 0:
         return o
     with _on(dev):
-        check(lib().mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
-                                             step.block_table.data_ptr(), step.width, step.cu_q.data_ptr(),
-                                             step.seq_lens.data_ptr(), step.requests, T, cfg.n_heads, cfg.n_kv_heads,
-                                             cfg.head_dim, cfg.v_head_dim, float(cfg.scale), cfg.window,
-                                             cfg.keep_first, cache.num_pages, cache.page_size, o.data_ptr(),
-                                             step.status.data_ptr(), _stream(dev)), "attention_paged")
+        L = lib()
+        nb = L.mimo_moe_paged_attention_workspace_bytes(T, cfg.n_heads, cfg.n_kv_heads, cfg.v_head_dim)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev)   # the call's own: two streams or graphs never share it
+        check(L.mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
+                                         step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,
+                                         cfg.n_kv_heads, cfg.head_dim, cfg.v_head_dim, float(cfg.scale), cfg.window,
+                                         cfg.keep_first, cache.num_pages, cache.page_size, plan.buffer.data_ptr(),
+                                         plan.buffer.numel(), o.data_ptr(), ws.data_ptr(), nb,
+                                         step.status.data_ptr(), _stream(dev)), "attention_paged")
     return o
 
 
@@ -353,8 +391,12 @@ class PagedDecoderStack(DecoderStack):
     def __call__(self, x: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
         _need_cuda(x, "x")
         step = self.table.step(new_lens, x.shape[0])
-        for c in self.caches:
-            c.step = step
+        plans = {}
+        for c in self.caches:   # one attention plan for each kind of layer
+            kind = _kind(c.cfg)
+            if kind not in plans:
+                plans[kind] = attention_plan(step, c.cfg)
+            c.step, c.plan = step, plans[kind]
         return super().__call__(x)
 
 

@@ -58,6 +58,41 @@ def test_paged_rope_store_refuses(bad):
     assert _lib().mimo_moe_paged_rope_store(*d.values()) == EINVAL
 
 
+@pytest.mark.parametrize("bad", [dict(cu=None), dict(seq=None), dict(plan=None), dict(R=0), dict(R=4097), dict(T=0),
+                                 dict(nq=0), dict(nkv=0), dict(nkv=3), dict(nq=258, nkv=2), dict(window=-1),
+                                 dict(keep=-1), dict(window=0, keep=4), dict(width=0), dict(P=8), dict(width=1 << 28),
+                                 dict(plan=A + 8), dict(nb=-1)])
+def test_paged_attention_plan_refuses(bad):
+    L = _lib()
+    d = dict(cu=A, seq=A, R=2, T=40, nq=8, nkv=2, window=128, keep=4, width=8, P=16, plan=A, nb=0, status=None,
+             stream=None)
+    d["nb"] = L.mimo_moe_paged_attention_plan_bytes(40, 2, 8, 2)
+    assert d["nb"] > 0
+    if bad.get("nb"):
+        bad = dict(nb=d["nb"] - 1)
+    d.update(bad)
+    assert L.mimo_moe_paged_attention_plan(*d.values()) == EINVAL
+
+
+@pytest.mark.parametrize("bad", [dict(q=None), dict(k=None), dict(v=None), dict(table=None), dict(plan=None),
+                                 dict(out=None), dict(ws=None), dict(R=0), dict(R=4097), dict(T=0), dict(nkv=3),
+                                 dict(nq=258, nkv=2), dict(d=96), dict(dv=192), dict(d=64), dict(scale=0.0),
+                                 dict(scale=float("nan")), dict(window=-1), dict(keep=-1), dict(window=0, keep=4),
+                                 dict(pages=0), dict(P=24), dict(width=0), dict(q=A + 8), dict(k=A + 2), dict(v=A + 8),
+                                 dict(out=A + 8), dict(plan=A + 4), dict(ws=A + 4), dict(nb=-1), dict(wb=-1),
+                                 dict(pages=1 << 26, nq=256, nkv=128, T=1)])
+def test_paged_attention_refuses(bad):
+    L = _lib()
+    d = dict(q=A, k=A, v=A, sinks=None, table=A, width=8, R=2, T=40, nq=8, nkv=2, d=192, dv=128, scale=0.1, window=128,
+             keep=4, pages=8, P=16, plan=A, nb=0, out=A, ws=A, wb=0, status=None, stream=None)
+    d.update({k: v for k, v in bad.items() if k not in ("nb", "wb")})
+    d["nb"] = max(0, L.mimo_moe_paged_attention_plan_bytes(40, 2, 8, 2)) + 10**9 - 10**9 * (("nb" in bad) or 0)
+    d["wb"] = 10**10 if "wb" not in bad else L.mimo_moe_paged_attention_workspace_bytes(40, 8, 2, 128) - 1
+    if "nb" in bad:
+        d["nb"] -= 1
+    assert L.mimo_moe_paged_attention(*d.values()) == EINVAL
+
+
 def test_python_checks_refuse():
     from mimo_moe import paged
     from mimo_moe.layer import AttentionConfig
