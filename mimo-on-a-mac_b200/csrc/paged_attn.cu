@@ -314,19 +314,31 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
-// MN-major operand, 128B swizzle: 64 contiguous values (128 B) along N per row of K, 8 rows per 1024-byte atom; LBO =
-// stride between groups of 64 values along N, SBO = stride between groups of 8 rows along K.
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 |
-         (uint64_t)((sbo >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-// kind::f16 with A in TMEM: lane = row of A, a 32-bit column holds two consecutive values along K.
-__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// Shared-memory matrix descriptors, 128B swizzle, 8-row groups 1024 bytes apart, sm_100 format: the upper word is the
+// same for both layouts, the lower one holds address / 16 (advanced by plain additions) and the leading byte offset:
+// unused for a K-major operand (Q, K), the stride between groups of 64 values along N for an MN-major one (V).
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t saddr) { return (saddr >> 4) | (1024u << 16); }
+// kind::f16 MMAs.  One thread issues them, and a product of K = 16 takes the tensor core 64 cycles, so the issue must
+// take fewer: the descriptors are put together from one changing word each.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
   asm volatile(
-      "{\n.reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "{\n.reg .pred p;\n.reg .b64 da, db;\n"
+      "setp.ne.u32 p, %4, 0;\n"
+      "mov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHi)
+      : "memory");
+}
+// A in TMEM: lane = row of A, a 32-bit column holds two consecutive values along K.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n.reg .pred p;\n.reg .b64 db;\n"
+      "setp.ne.u32 p, %4, 0;\n"
+      "mov.b64 db, {%2, %5};\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHi)
       : "memory");
 }
 
@@ -336,6 +348,7 @@ template <int DQK, int DV>
 struct Shape {
   static constexpr int QCH = DQK / 64, VCH = DV / 64;
   static constexpr uint32_t QB = 128u * DQK * 2;
+  static constexpr int NG = 16;  // barriers of K and V blocks: more than the ring holds (12 chunks at most)
   static constexpr int NS = (int)((232448u - 2048u - 2 * QB) / kChunk);  // ring slots in what Q leaves
   static constexpr uint32_t SMEM = 2048 + 2 * QB + NS * kChunk;          // barriers, alignment slack, tiles
 };
@@ -347,12 +360,12 @@ struct Seg {
 template <int DQK, int DV>
 __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
   using S = Shape<DQK, DV>;
-  constexpr int NS = S::NS, CPB = S::QCH + S::VCH;  // ring slots, chunks per block
+  constexpr int NS = S::NS, NG = S::NG, CPB = S::QCH + S::VCH;  // ring slots, block barriers, chunks per block
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
-  uint64_t* full = bars;
-  uint64_t* empty = full + NS;
-  uint64_t* q_full = empty + NS;
+  uint64_t* full = bars;  // K_j is block 2 j of the ring, V_j block 2 j + 1
+  uint64_t* empty = full + NG;
+  uint64_t* q_full = empty + NG;
   uint64_t* q_empty = q_full + 2;
   uint64_t* s_full = q_empty + 2;
   uint64_t* p_full = s_full + 2;
@@ -367,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NS; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < NG; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
@@ -414,7 +427,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const uint64_t pol = tc::l2_evict_normal_policy();
       const int P = 1 << p.page_shift, ppb = 128 >> p.page_shift;  // pages per block
       const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
-      uint32_t ci = 0;                                             // chunks issued
+      uint32_t ci = 0, nb = 0;                                     // chunks and key blocks issued
+      uint32_t freed = 0;                                          // ring blocks known to be free again
       uint32_t nq[2] = {0, 0};                                     // Q loads of each tile
       for (int s = 0; s < nseg && ok; ++s) {
         const Seg g = load_seg(s);
@@ -453,28 +467,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
                 }
               }
             }
-            const uint32_t sl = ci % NS;
-            if (ok) ok = mbar_wait(&empty[sl], ((ci / NS) & 1) ^ 1);
+            if (ci >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
+              const uint32_t old = ci - NS, g = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
+              if (ok && g >= freed) ok = mbar_wait(&empty[g % NG], (g / NG) & 1);
+              freed = g + 1;
+            }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&full[sl], kChunk);
-            __syncwarp();
+            const uint32_t sl = ci % NS;
+            uint64_t* bar = &full[(2 * nb + (c >= S::QCH ? 1 : 0)) % NG];
+            if (c == 0 || c == S::QCH) {
+              if (lane == 0) mbar_arrive_expect_tx(bar, (c == 0 ? S::QCH : S::VCH) * kChunk);
+              __syncwarp();
+            }
             if (lane < ppb) {
               uint8_t* dst = sRing + sl * kChunk + (uint32_t)lane * P * 128;
               if (c < S::QCH)
-                tma_load_3d(dst, &p.kmap, c * 64, 0, row, &full[sl], pol);
+                tma_load_3d(dst, &p.kmap, c * 64, 0, row, bar, pol);
               else
-                tma_load_3d(dst, &p.vmap, (c - S::QCH) * 64, 0, row, &full[sl], pol);
+                tma_load_3d(dst, &p.vmap, (c - S::QCH) * 64, 0, row, bar, pol);
             }
             ++ci;
           }
+          ++nb;
           row = next;
         }
       }
-      // no copy may still be landing when the CTA exits: the last chunk of every slot, and Q
-      for (uint32_t k = 0; k < (uint32_t)NS && k < ci; ++k) {
-        const uint32_t i = ci - 1 - k;
-        mbar_wait(&full[i % NS], (i / NS) & 1);
+      // no copy may still be landing when the CTA exits: the last blocks (after a wait that ran out, what there is of
+      // the block it was in: these waits run out too), and Q
+      if (!ok) mbar_wait(&full[(2 * nb) % NG], (2 * nb / NG) & 1), mbar_wait(&full[(2 * nb + 1) % NG], ((2 * nb + 1) / NG) & 1);
+      for (uint32_t k = 0; k < (uint32_t)NG && k < 2 * nb; ++k) {
+        const uint32_t i = 2 * nb - 1 - k;
+        mbar_wait(&full[i % NG], (i / NG) & 1);
       }
       for (int x = 0; x < 2; ++x)
         if (nq[x]) mbar_wait(&q_full[x], (nq[x] - 1) & 1);
@@ -483,86 +507,87 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const uint32_t idesc_s = tc::idesc_bf16(128, 128);
         const uint32_t idesc_o64 = tc::idesc_bf16(128, 64) | (1u << 16);  // B = V, MN-major
         const uint32_t idesc_o = tc::idesc_bf16(128, DV) | (1u << 16);
-        const uint32_t aq = smem_u32(sQ), ar = smem_u32(sRing);
-        uint32_t ci = 0;  // chunks of the blocks before this one
-        uint32_t ns[2] = {0, 0}, np[2] = {0, 0}, fixes = 0;
-        auto chunks_there = [&](uint32_t at, int n) {
-          for (int c = 0; c < n && ok; ++c) ok = mbar_wait(&full[(at + c) % NS], ((at + c) / NS) & 1);
+        const uint32_t aq = desc_k(smem_u32(sQ)), bk = desc_k(smem_u32(sRing)), bv = desc_mn(smem_u32(sRing));
+        uint32_t nb = 0, slot = 0;  // key blocks before this one, ring slot of its first chunk
+        uint32_t nq[2] = {0, 0}, np[2] = {0, 0}, fixes = 0;
+        auto there = [&](uint32_t g) {
+          if (ok) ok = mbar_wait(&full[g % NG], (g / NG) & 1);
           tc::tc_fence_after();
         };
-        // S = Q K^T of tile x from the K chunks at ring position `at`; the last tile to read them frees each
-        auto issue_s = [&](int x, uint32_t at, bool frees) {
+        auto wrap = [](uint32_t sl) -> uint32_t { return sl >= (uint32_t)NS ? sl - NS : sl; };
+        // S = Q K^T of tile x from the K chunks at ring slot `at`
+        auto issue_s = [&](int x, uint32_t at) {
+          const uint32_t d = tbase + x * 128;
 #pragma unroll
           for (int c = 0; c < S::QCH; ++c) {
-            const uint32_t sl = (at + c) % NS;
+            const uint32_t a = aq + (x * S::QB + c * kChunk) / 16, b = bk + wrap(at + c) * (kChunk / 16);
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              tc::tc_mma_f16(tbase + x * 128, tc::desc_sw128(aq + x * S::QB + c * kChunk + kk * 32),
-                             tc::desc_sw128(ar + sl * kChunk + kk * 32), idesc_s, (c | kk) != 0 ? 1u : 0u);
-            if (frees) tc::tc_commit(&empty[sl]);
+            for (int kk = 0; kk < 4; ++kk) mma_ss(d, a + kk * 2, b + kk * 2, idesc_s, (c | kk) != 0);
           }
           tc::tc_commit(&s_full[x]);
         };
-        auto issue_pv = [&](int x, uint32_t at, bool first, bool frees) {
+        // O += P V of tile x from the V chunks at ring slot `at`
+        auto issue_pv = [&](int x, uint32_t at, bool first) {
           const uint32_t d = tbase + 256 + x * DV, a = tbase + x * 128;
-          const uint32_t sl = at % NS;
-          if (S::VCH == 2 && sl + 1 < (uint32_t)NS) {  // the two V chunks lie one behind the other
+          if (S::VCH == 1 || at + 1 < (uint32_t)NS) {  // the V chunks lie one behind the other
+            const uint32_t b = bv + at * (kChunk / 16);
 #pragma unroll
-            for (int kk = 0; kk < 8; ++kk)
-              tc_mma_f16_ts(d, a + kk * 8, desc_mn_sw128(ar + sl * kChunk + kk * 2048, kChunk, 1024), idesc_o,
-                            (!first || kk != 0) ? 1u : 0u);
+            for (int kk = 0; kk < 8; ++kk) mma_ts(d, a + kk * 8, b + kk * 128, idesc_o, kk != 0 || !first);
           } else {
 #pragma unroll
-            for (int c = 0; c < S::VCH; ++c)
+            for (int c = 0; c < S::VCH; ++c) {
+              const uint32_t b = bv + wrap(at + c) * (kChunk / 16);
 #pragma unroll
-              for (int kk = 0; kk < 8; ++kk)
-                tc_mma_f16_ts(d + c * 64, a + kk * 8,
-                              desc_mn_sw128(ar + ((at + c) % NS) * kChunk + kk * 2048, kChunk, 1024), idesc_o64,
-                              (!first || kk != 0) ? 1u : 0u);
+              for (int kk = 0; kk < 8; ++kk) mma_ts(d + c * 64, a + kk * 8, b + kk * 128, idesc_o64, kk != 0 || !first);
+            }
           }
-          if (frees)
-            for (int c = 0; c < S::VCH; ++c) tc::tc_commit(&empty[(at + c) % NS]);
         };
         for (int s = 0; s < nseg && ok; ++s) {
           const Seg g = load_seg(s);
           const int qlast = g.qfirst + g.ntok - 1;
           const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
-          const int nx = g.ntok > tpt ? 2 : 1;
-          chunks_there(ci, S::QCH);
-          for (int x = 0; x < nx && ok; ++x) {
-            ok = mbar_wait(&q_full[x], ns[x] & 1);
-            ++ns[x];
-            tc::tc_fence_after();
+          const bool pair = g.ntok > tpt;
+          there(2 * nb);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (x == 1 && !pair) break;
+            if (ok) ok = mbar_wait(&q_full[x], nq[x] & 1);
+            ++nq[x];
             if (!ok) break;
-            issue_s(x, ci, x == nx - 1);
+            tc::tc_fence_after();
+            issue_s(x, slot);
             if (g.nblk == 1) tc::tc_commit(&q_empty[x]);
           }
-          for (int j = 0; j < g.nblk && ok; ++j) {
+          tc::tc_commit(&empty[(2 * nb) % NG]);
+          for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
             const int kb = g.b0 + j < bl.nkb ? g.b0 + j : bl.lb + (g.b0 + j - bl.nkb);
             const int kp = kb * 128;
-            const uint32_t at = ci + S::QCH;
+            const uint32_t vs = wrap(slot + S::QCH), next = wrap(vs + S::VCH);
+            const bool more = j + 1 < g.nblk;
             // some rows of V are nobody's: zeroed while the softmax runs
             const bool fix = !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
-            chunks_there(at, S::VCH);
+            there(2 * nb + 1);
             if (fix && ok) mbar_arrive(fix_req);
-            const bool more = j + 1 < g.nblk;
-            for (int x = 0; x < nx && ok; ++x) {
-              ok = mbar_wait(&p_full[x], np[x] & 1);
+            if (more) there(2 * nb + 2);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (x == 1 && !pair) break;
+              if (ok) ok = mbar_wait(&p_full[x], np[x] & 1);
               ++np[x];
               if (x == 0 && fix && ok) ok = mbar_wait(v_fixed, fixes++ & 1);
-              tc::tc_fence_after();
               if (!ok) break;
-              issue_pv(x, at, j == 0, x == nx - 1);
+              tc::tc_fence_after();
+              issue_pv(x, vs, j == 0);
+              if (x == (pair ? 1 : 0)) tc::tc_commit(&empty[(2 * nb + 1) % NG]);
               if (more) {
-                if (x == 0) chunks_there(ci + CPB, S::QCH);
-                if (!ok) break;
-                issue_s(x, ci + CPB, x == nx - 1);
+                issue_s(x, next);
+                if (x == (pair ? 1 : 0)) tc::tc_commit(&empty[(2 * nb + 2) % NG]);
                 if (j + 2 == g.nblk) tc::tc_commit(&q_empty[x]);
               } else {
                 tc::tc_commit(&o_full[x]);
               }
             }
-            ci += CPB;
+            slot = next;
           }
         }
         tc::tc_commit(drain);  // every MMA issued above has completed once this arrives
@@ -611,8 +636,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const Blocks bl = blocks_of(g.qfirst, g.qfirst + g.ntok - 1, p.window, p.keep);
       const bool row_ok = r < tpt * p.G && tt < g.ntok;
       const bool work = __any_sync(0xFFFFFFFFu, row_ok);  // a warp without a row only keeps the barriers going
-      const int qpos = row_ok ? g.qfirst + tt : -1;
-      const int lo = p.window > 0 ? max(0, qpos - p.window + 1) : 0;
+      // rows without a query compute on what lies there, unmasked: nobody reads their results
+      const int qpos = row_ok ? g.qfirst + tt : 0x7FFFFFFF;
+      const int lo = p.window > 0 && row_ok ? max(0, qpos - p.window + 1) : 0;
       const int keep = min(p.keep, lo);
       float m_ref = -INFINITY, l = 0.f;
       for (int j = 0; j < g.nblk; ++j) {
@@ -628,10 +654,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           tc::tmem_wait_ld();
           const int jb = g.b0 + j, kp = (jb < bl.nkb ? jb : bl.lb + (jb - bl.nkb)) * 128;
           if (!(kp + 127 <= qpos && (kp >= lo || kp + 127 < keep))) {
+            // 32 columns at a time as a word of visible bits: [c_lo, c_hi] and [0, c_keep)
             const int c_hi = qpos - kp, c_lo = lo - kp, c_keep = keep - kp;
 #pragma unroll
-            for (int c = 0; c < 128; ++c)
-              if (c > c_hi || (c < c_lo && c >= c_keep)) v[c] = -INFINITY;
+            for (int w = 0; w < 4; ++w) {
+              auto below = [&](int c) -> uint32_t {  // bits of the columns < c
+                const int k = min(max(c - w * 32, 0), 32);
+                return k == 32 ? 0xFFFFFFFFu : (1u << k) - 1u;
+              };
+              const uint32_t seen = below(min(c_hi, 0x7FFFFFFE) + 1) & (~below(c_lo) | below(c_keep));
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (!(seen & (1u << e))) v[w * 32 + e] = -INFINITY;
+            }
           }
           float mx[4];
 #pragma unroll
