@@ -2,10 +2,12 @@
 // cores: a plan of the step's work (one small launch, shared by all layers of a kind), the attention kernel (one
 // persistent CTA per SM) and the merge of what was split.
 //
-// A work unit is one kv head of up to 2 * (128 / G) consecutive new tokens of one request: two tiles A and B of 128
-// query rows (the G = n_heads / n_kv_heads heads of 128 / G tokens, token-major, so that one K/V block serves the whole
-// group and both tiles), over the blocks of 128 key positions that its queries see: blocks 0 .. nkb - 1 hold the first
-// tokens that stay visible, blocks lb .. the window (all, without one).
+// A work unit is one kv head of up to 2 * (128 / G) consecutive new tokens of one request, over the blocks of 128 key
+// positions that its queries see: blocks 0 .. nkb - 1 hold the first tokens that stay visible, blocks lb .. the window
+// (all, without one).  A tile is 128 query rows, the G = n_heads / n_kv_heads heads of 128 / G tokens, token-major, so
+// that one K/V block serves the whole group.  A unit of more than one tile (a pair) works on two, A and B, over the same
+// blocks.  A unit of one tile (a decoding request's) works on its even blocks as A and on its odd ones as B, and joins
+// the two at its end.  Either way the two softmax groups and the MMAs take turns, so neither waits out the other.
 //
 // One CTA, 12 warps:
 //   warps 0-3, 4-7   softmax of tile A and of tile B, one thread per query row (TMEM lane = row): the 128 scores of S_j
@@ -17,8 +19,8 @@
 //                    one ring of shared-memory slots; lane i copies the i-th page of the block (a box of 64 dims x
 //                    page_size positions), and pages nobody sees are read as zeros from behind the pool's end;
 //   warp 9           MMA issuer (one thread): S = Q K^T and O += P V, alternating the tiles, so that one tile's products
-//                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV_j and
-//                    S_j+1 are issued in this order, so when S_j+1 is there, O holds PV_j and P_j is consumed;
+//                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV and its
+//                    next S are issued in this order, so when that S is there, O holds PV and P is consumed;
 //   warp 10          zeroes the V rows that no query of the unit sees in the blocks at the range's ends: such slots may
 //                    hold anything, and 0 * NaN is not 0.
 // Every wait is bounded and sets MIMO_ETIMEOUT; the producer drains its copies and the issuer its MMAs before exit.
@@ -81,6 +83,8 @@ __device__ __forceinline__ Blocks blocks_of(int qfirst, int qlast, int window, i
 
 constexpr int kPlanThreads = 1024;
 constexpr int kBuckets = 2048;
+// What a unit costs besides its blocks (Q, the first scores, the epilogue), in blocks.
+constexpr int kUnitCost = 2;
 
 __device__ __forceinline__ long long block_scan(long long v, long long* excl, long long* sh) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -106,7 +110,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* excl, lo
 
 // One CTA.  Two ways to deal the units to the n CTAs: whole units, longest first, in a snake (no partial results), or
 // the units' blocks one after another in n equal ranges (perfect balance; a unit cut by a range's end leaves partial
-// results that the merge kernel joins).  The one whose longest CTA takes less is taken, in units of a key block.
+// results that the merge kernel joins).  The one whose longest CTA takes less is taken, in units of a key block, each
+// unit counted as its blocks and kUnitCost more.
 __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams p) {
   extern __shared__ int sm[];
   int* toff = sm;                       // [R + 1] tiles before request r
@@ -175,12 +180,12 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
       tiles[i] = make_int4(a + t0, ntok, qfirst, r);
       nbs[i] = nb;
       atomicAdd(&hist[kBuckets - 1 - min(nb, kBuckets - 1)], 1);
-      mine += nb;
+      mine += nb + kUnitCost;
     }
     W = block_scan(mine, &ex, sh);
     for (int i = i0; i < i1; ++i) {
       pre[i] = ex;
-      ex += nbs[i];
+      ex += nbs[i] + kUnitCost;
     }
     if (tid == 0) pre[nt] = W;
   }
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     const int k = u / n, c = u % n;
     return (k & 1) ? n - 1 - c : c;
   };
-  for (int u = tid; u < units; u += kPlanThreads) atomicAdd(&load[cta_of(u)], nbs[order[u / p.nkv]] + 1);
+  for (int u = tid; u < units; u += kPlanThreads) atomicAdd(&load[cta_of(u)], nbs[order[u / p.nkv]] + kUnitCost);
   __syncthreads();
   int most = tid < n ? load[tid] : 0;
 #pragma unroll
@@ -219,8 +224,8 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
   __syncthreads();
   for (int w = 0; w < kPlanThreads / 32; ++w) most = max(most, load[w]);
   // a CTA's range holds at least two blocks: a shorter one costs more in its partial result than it saves
-  const long long quota = max(2ll, (W + n - 1) / n);
-  const bool split = quota + (units + n - 1) / n + p.merge_cost < most;
+  const long long quota = max(2ll + kUnitCost, (W + n - 1) / n);
+  const bool split = quota + p.merge_cost < most;
   if (tid == 0) {
     p.plan[1] = units;
     p.plan[2] = split ? 1 : 0;
@@ -237,18 +242,23 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     } else if (c * quota >= W) {
       base[c] = 0, cnt[c] = 0;
     } else {
-      // the unit that holds block x of the line of all units' blocks
+      // the unit that holds x on the line of all units' costs, and where its first block lies (its own cost comes before)
+      long long first_block;
       auto unit_at = [&](long long x) -> int {
         int lo = 0, hi = nt - 1;
         while (lo < hi) {
           const int mid = (lo + hi + 1) >> 1;
           if (pre[mid] * p.nkv <= x) lo = mid; else hi = mid - 1;
         }
-        return lo * p.nkv + (int)((x - pre[lo] * p.nkv) / nbs[lo]);
+        const int len = nbs[lo] + kUnitCost, hk = (int)((x - pre[lo] * p.nkv) / len);
+        first_block = pre[lo] * p.nkv + (long long)hk * len + kUnitCost;
+        return lo * p.nkv + hk;
       };
-      const int first = unit_at(c * quota), last = unit_at(min(W, (c + 1) * quota) - 1);
+      const long long end = min(W, (c + 1) * quota);
+      const int first = unit_at(c * quota) + (first_block >= end ? 1 : 0);
+      const int last = unit_at(end - 1) - (first_block >= end ? 1 : 0);
       base[c] = first + c;
-      cnt[c] = last - first + 1;
+      cnt[c] = max(0, last - first + 1);
     }
   }
   __syncthreads();
@@ -261,7 +271,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     } else {
       const int i = u / p.nkv, hk = u % p.nkv, nb = nbs[i];
       const int4 t = tiles[i];
-      const long long s0 = pre[i] * p.nkv + (long long)hk * nb, s1 = s0 + nb;
+      const long long s0 = pre[i] * p.nkv + (long long)hk * (nb + kUnitCost) + kUnitCost, s1 = s0 + nb;  // its blocks
       const int c0 = (int)(s0 / quota), c1 = (int)((s1 - 1) / quota);
       int slot0 = -1;
       for (int c = c0; c <= c1; ++c) {
@@ -342,6 +352,8 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
+constexpr uint32_t kHead = 1024 + 2048;  // barriers, the exchange between the softmax groups; tiles start at a multiple
+                                         // of 1024 bytes, as the block's shared memory does
 constexpr uint32_t kChunk = 16384;  // 128 positions x 64 dims, bf16
 
 template <int DQK, int DV>
@@ -349,8 +361,10 @@ struct Shape {
   static constexpr int QCH = DQK / 64, VCH = DV / 64;
   static constexpr uint32_t QB = 128u * DQK * 2;
   static constexpr int NG = 16;  // barriers of K and V blocks: more than the ring holds (12 chunks at most)
-  static constexpr int NS = (int)((232448u - 2048u - 2 * QB) / kChunk);  // ring slots in what Q leaves
-  static constexpr uint32_t SMEM = 2048 + 2 * QB + NS * kChunk;          // barriers, alignment slack, tiles
+  static constexpr int NS = (int)((232448u - kHead - 2 * QB) / kChunk);  // ring slots in what Q leaves
+  static constexpr uint32_t SMEM = kHead + 2 * QB + NS * kChunk;
+  // a single tile's second K block is read before its first V block leaves the ring
+  static_assert(2 * QCH + VCH <= NS, "the ring must hold K, V and the next K");
 };
 
 struct Seg {
@@ -374,9 +388,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   uint64_t* v_fixed = fix_req + 1;
   uint64_t* drain = v_fixed + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
-  uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)(smem + 1024) + 1023) & ~(uintptr_t)1023);
-  uint8_t* sQ = base;
-  uint8_t* sRing = base + 2 * S::QB;
+  float2* xchg = reinterpret_cast<float2*>(smem + 1024);  // [2][128] (maximum, sum) of the tiles' rows
+  uint8_t* sQ = smem + kHead;
+  uint8_t* sRing = sQ + 2 * S::QB;
+  if (smem_u32(smem) & 1023) {  // never seen: the swizzled tiles would be read wrongly
+    if (threadIdx.x == 0) set_status(p.status, MIMO_EINVAL);
+    return;
+  }
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -429,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
       uint32_t ci = 0, nb = 0;                                     // chunks and key blocks issued
       uint32_t freed = 0;                                          // ring blocks known to be free again
-      uint32_t nq[2] = {0, 0};                                     // Q loads of each tile
+      uint32_t nq = 0, turn = 0;                                   // phases of the Q buffers, the next single tile's
       for (int s = 0; s < nseg && ok; ++s) {
         const Seg g = load_seg(s);
         const int qlast = g.qfirst + g.ntok - 1;
@@ -452,20 +470,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           const int next = j + 1 < g.nblk ? page_of(g.b0 + j + 1) : 0;
 #pragma unroll
           for (int c = 0; c < CPB; ++c) {
-            if (c == S::QCH && j == 0) {  // Q behind the first K block
+            if (c == S::QCH && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
+              const bool pair = g.ntok > tpt;
 #pragma unroll
               for (int x = 0; x < 2; ++x) {
-                if (x == 1 && g.ntok <= tpt) break;
-                if (ok) ok = mbar_wait(&q_empty[x], (nq[x] & 1) ^ 1);
-                ++nq[x];
+                const int qb = pair ? x : turn;
+                if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
+                nq ^= 1u << qb;
                 if (lane == 0 && ok) {
-                  mbar_arrive_expect_tx(&q_full[x], (uint32_t)(S::QCH * 128 * p.G * tpt));
+                  mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
 #pragma unroll
                   for (int d = 0; d < S::QCH; ++d)
-                    tma_load_3d(sQ + x * S::QB + d * kChunk, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[x],
-                                pol);
+                    tma_load_3d(sQ + qb * S::QB + d * kChunk, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt,
+                                &q_full[qb], pol);
                 }
+                if (!pair) break;
               }
+              if (!pair) turn ^= 1;
             }
             if (ci >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
               const uint32_t old = ci - NS, g = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
@@ -500,8 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const uint32_t i = 2 * nb - 1 - k;
         mbar_wait(&full[i % NG], (i / NG) & 1);
       }
-      for (int x = 0; x < 2; ++x)
-        if (nq[x]) mbar_wait(&q_full[x], (nq[x] - 1) & 1);
+      for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
     } else if (warp == 9) {
       if (lane == 0) {  // ------------------------------------------------------------------------- MMA issuer
         const uint32_t idesc_s = tc::idesc_bf16(128, 128);
@@ -509,18 +529,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const uint32_t idesc_o = tc::idesc_bf16(128, DV) | (1u << 16);
         const uint32_t aq = desc_k(smem_u32(sQ)), bk = desc_k(smem_u32(sRing)), bv = desc_mn(smem_u32(sRing));
         uint32_t nb = 0, slot = 0;  // key blocks before this one, ring slot of its first chunk
-        uint32_t nq[2] = {0, 0}, np[2] = {0, 0}, fixes = 0;
+        uint32_t nq = 0, turn = 0, np = 0, nfix = 0;  // phases
         auto there = [&](uint32_t g) {
           if (ok) ok = mbar_wait(&full[g % NG], (g / NG) & 1);
           tc::tc_fence_after();
         };
         auto wrap = [](uint32_t sl) -> uint32_t { return sl >= (uint32_t)NS ? sl - NS : sl; };
-        // S = Q K^T of tile x from the K chunks at ring slot `at`
-        auto issue_s = [&](int x, uint32_t at) {
+        auto q_there = [&](int qb) {
+          if (ok) ok = mbar_wait(&q_full[qb], (nq >> qb) & 1);
+          nq ^= 1u << qb;
+          tc::tc_fence_after();
+        };
+        auto p_there = [&](int x) {
+          if (ok) ok = mbar_wait(&p_full[x], (np >> x) & 1);
+          np ^= 1u << x;
+        };
+        auto fixed = [&]() {
+          if (ok) ok = mbar_wait(v_fixed, nfix & 1);
+          ++nfix;
+        };
+        // S = Q K^T of tile x from Q buffer qb and the K chunks at ring slot `at`
+        auto issue_s = [&](int x, int qb, uint32_t at) {
           const uint32_t d = tbase + x * 128;
 #pragma unroll
           for (int c = 0; c < S::QCH; ++c) {
-            const uint32_t a = aq + (x * S::QB + c * kChunk) / 16, b = bk + wrap(at + c) * (kChunk / 16);
+            const uint32_t a = aq + (qb * S::QB + c * kChunk) / 16, b = bk + wrap(at + c) * (kChunk / 16);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) mma_ss(d, a + kk * 2, b + kk * 2, idesc_s, (c | kk) != 0);
           }
@@ -546,48 +579,79 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           const Seg g = load_seg(s);
           const int qlast = g.qfirst + g.ntok - 1;
           const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
-          const bool pair = g.ntok > tpt;
-          there(2 * nb);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (x == 1 && !pair) break;
-            if (ok) ok = mbar_wait(&q_full[x], nq[x] & 1);
-            ++nq[x];
-            if (!ok) break;
-            tc::tc_fence_after();
-            issue_s(x, slot);
-            if (g.nblk == 1) tc::tc_commit(&q_empty[x]);
-          }
-          tc::tc_commit(&empty[(2 * nb) % NG]);
-          for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
-            const int kb = g.b0 + j < bl.nkb ? g.b0 + j : bl.lb + (g.b0 + j - bl.nkb);
-            const int kp = kb * 128;
-            const uint32_t vs = wrap(slot + S::QCH), next = wrap(vs + S::VCH);
-            const bool more = j + 1 < g.nblk;
-            // some rows of V are nobody's: zeroed while the softmax runs
-            const bool fix = !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
-            there(2 * nb + 1);
-            if (fix && ok) mbar_arrive(fix_req);
-            if (more) there(2 * nb + 2);
+          // block j of the unit has V rows that are nobody's
+          auto ragged = [&](int j) -> bool {
+            const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb), kp = kb * 128;
+            return !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
+          };
+          if (g.ntok > tpt) {  // a pair: both tiles on every block
+            there(2 * nb);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              if (x == 1 && !pair) break;
-              if (ok) ok = mbar_wait(&p_full[x], np[x] & 1);
-              ++np[x];
-              if (x == 0 && fix && ok) ok = mbar_wait(v_fixed, fixes++ & 1);
+              q_there(x);
+              if (!ok) break;
+              issue_s(x, x, slot);
+              if (g.nblk == 1) tc::tc_commit(&q_empty[x]);
+            }
+            tc::tc_commit(&empty[(2 * nb) % NG]);
+            for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
+              const uint32_t vs = wrap(slot + S::QCH), next = wrap(vs + S::VCH);
+              const bool more = j + 1 < g.nblk, fix = ragged(g.b0 + j);
+              there(2 * nb + 1);
+              if (fix && ok) mbar_arrive(fix_req);  // zeroed while the softmax runs
+              if (more) there(2 * nb + 2);
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                p_there(x);
+                if (x == 0 && fix) fixed();
+                if (!ok) break;
+                tc::tc_fence_after();
+                issue_pv(x, vs, j == 0);
+                if (x == 1) tc::tc_commit(&empty[(2 * nb + 1) % NG]);
+                if (more) {
+                  issue_s(x, x, next);
+                  if (x == 1) tc::tc_commit(&empty[(2 * nb + 2) % NG]);
+                  if (j + 2 == g.nblk) tc::tc_commit(&q_empty[x]);
+                } else {
+                  tc::tc_commit(&o_full[x]);
+                }
+              }
+              slot = next;
+            }
+          } else {  // one tile: blocks in turn as A and B
+            const uint32_t qb = turn;
+            turn ^= 1;
+            const uint32_t nb0 = nb;
+            uint32_t ks = slot, kb = nb;  // the next block whose S is issued
+            auto issue_next = [&](int x) {
+              there(2 * kb);
+              if (!ok) return;
+              issue_s(x, qb, ks);
+              tc::tc_commit(&empty[(2 * kb) % NG]);
+              ks = wrap(ks + CPB);
+              if (++kb == nb0 + g.nblk) tc::tc_commit(&q_empty[qb]);
+            };
+            q_there(qb);
+            issue_next(0);
+            if (g.nblk > 1) issue_next(1);
+            for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
+              const int x = j & 1;
+              const uint32_t vs = wrap(slot + S::QCH);
+              const bool fix = ragged(g.b0 + j);
+              there(2 * nb + 1);
+              if (fix && ok) mbar_arrive(fix_req);
+              p_there(x);
+              if (fix) fixed();
               if (!ok) break;
               tc::tc_fence_after();
-              issue_pv(x, vs, j == 0);
-              if (x == (pair ? 1 : 0)) tc::tc_commit(&empty[(2 * nb + 1) % NG]);
-              if (more) {
-                issue_s(x, next);
-                if (x == (pair ? 1 : 0)) tc::tc_commit(&empty[(2 * nb + 2) % NG]);
-                if (j + 2 == g.nblk) tc::tc_commit(&q_empty[x]);
-              } else {
-                tc::tc_commit(&o_full[x]);
-              }
+              issue_pv(x, vs, j < 2);
+              tc::tc_commit(&empty[(2 * nb + 1) % NG]);
+              // this block's V may have to leave the ring before that K can come
+              if (j + 2 < g.nblk) issue_next(x);
+              slot = wrap(vs + S::VCH);
             }
-            slot = next;
+            tc::tc_commit(&o_full[0]);
+            tc::tc_commit(&o_full[1]);
           }
         }
         tc::tc_commit(drain);  // every MMA issued above has completed once this arrives
@@ -627,12 +691,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     const int x = warp >> 2, r = threadIdx.x & 127;
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tbase + x * 128 + lane_off, tO = tbase + 256 + x * DV + lane_off;
-    const int tt = r / p.G + x * tpt, head = r % p.G;  // this row's token of the unit and head of the group
+    const int head = r % p.G;  // this row's head of the group
     const float sl2 = p.scale_log2;
     uint32_t ns = 0, no = 0;
-    for (int s = 0; s < nseg && ok; ++s) {
+    for (int s = 0; s < nseg; ++s) {
       const Seg g = load_seg(s);
-      if (x == 1 && g.ntok <= tpt) continue;
+      const bool pair = g.ntok > tpt;
+      const int tt = r / p.G + (pair ? x * tpt : 0);  // its token of the unit
       const Blocks bl = blocks_of(g.qfirst, g.qfirst + g.ntok - 1, p.window, p.keep);
       const bool row_ok = r < tpt * p.G && tt < g.ntok;
       const bool work = __any_sync(0xFFFFFFFFu, row_ok);  // a warp without a row only keeps the barriers going
@@ -641,11 +706,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int lo = p.window > 0 && row_ok ? max(0, qpos - p.window + 1) : 0;
       const int keep = min(p.keep, lo);
       float m_ref = -INFINITY, l = 0.f;
-      for (int j = 0; j < g.nblk; ++j) {
+      // after a wait that ran out the loops go on without work, for the barriers that both groups must pass
+      for (int j = pair ? 0 : x; j < g.nblk; j += pair ? 1 : 2) {
         if (ok) ok = mbar_wait(&s_full[x], ns & 1);
         ++ns;
         ok = __all_sync(0xFFFFFFFFu, ok);
-        if (!ok) break;
+        if (!ok) continue;
         tc::tc_fence_after();
         if (work) {
           float v[128];
@@ -720,52 +786,73 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (ok) ok = mbar_wait(&o_full[x], no & 1);
       ++no;
       ok = __all_sync(0xFFFFFFFFu, ok);
-      if (!ok) break;
+      // this thread's columns of the row, and the weights of the two outputs they are joined from (a pair's have one)
+      int c0 = 0, c1 = DV;
+      float w_own = 1.f, w_other = 0.f;
+      bool own = true, other = false;  // whether there is such an output (one never written may hold anything)
+      if (!pair) {
+        xchg[x * 128 + r] = make_float2(m_ref, l);
+        named_bar_sync(1, 256);
+        const float2 o = xchg[(x ^ 1) * 128 + r];
+        const float M = fmaxf(m_ref, o.x);
+        own = m_ref != -INFINITY || l != 0.f, other = o.x != -INFINITY || o.y != 0.f;
+        w_own = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
+        w_other = o.x == -INFINITY ? 0.f : exp2f(o.x - M);
+        l = l * w_own + o.y * w_other;
+        m_ref = M;
+        c0 = x * (DV / 2), c1 = c0 + DV / 2;
+      }
       tc::tc_fence_after();
-      if (!work) continue;
-      const int qh = g.hk * p.G + head, row = g.row0 + tt;
-      if (g.slot < 0) {
-        float f;
-        if (p.sinks) {
-          const float sk = (row_ok ? p.sinks[qh] : 0.f) * kLog2e;
-          const float M = fmaxf(m_ref, sk);
-          const float a = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
-          f = a / (l * a + exp2f(sk - M));
-        } else {
-          f = l > 0.f ? 1.f / l : 0.f;
+      if (work && ok) {
+        const int qh = g.hk * p.G + head, row = g.row0 + tt;
+        const uint32_t tOther = tbase + 256 + (x ^ 1) * DV + lane_off;
+        float f = 1.f;  // an unnormalised part: maximum (log2), sum and output of these blocks
+        if (g.slot < 0) {
+          if (p.sinks) {
+            const float sk = (row_ok ? p.sinks[qh] : 0.f) * kLog2e;
+            const float M = fmaxf(m_ref, sk);
+            const float a = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
+            f = a / (l * a + exp2f(sk - M));
+          } else {
+            f = l == 0.f ? 0.f : 1.f / l;
+          }
         }
-        uint16_t* dst = p.out + ((size_t)row * p.nq + qh) * DV;
+        w_own *= f, w_other *= f;
+        const bool store = row_ok && row < p.T;
+        const size_t at = (size_t)max(g.slot, 0) * p.part_rows + (tt * p.G + head);
 #pragma unroll 1
-        for (int c = 0; c < DV; c += 32) {
+        for (int c = c0; c < c1; c += 32) {
           float o[32];
           tmem_ld32(tO + c, o);
           tc::tmem_wait_ld();
-          if (row_ok && row < p.T) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = own ? o[e] * w_own : 0.f;
+          if (!pair) {
+            float q[32];
+            tmem_ld32(tOther + c, q);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
+          }
+          if (store && g.slot < 0) {
+            uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.nq + qh) * DV + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               uint32_t w[4];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2_rn(o[e * 8 + 2 * k] * f, o[e * 8 + 2 * k + 1] * f);
-              reinterpret_cast<uint4*>(dst + c)[e] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2_rn(o[e * 8 + 2 * k], o[e * 8 + 2 * k + 1]);
+              dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
             }
-          }
-        }
-      } else {  // an unnormalised part: maximum (log2), sum and output of these blocks
-        const size_t at = (size_t)g.slot * p.part_rows + (tt * p.G + head);
-#pragma unroll 1
-        for (int c = 0; c < DV; c += 32) {
-          float o[32];
-          tmem_ld32(tO + c, o);
-          tc::tmem_wait_ld();
-          if (row_ok) {
+          } else if (store) {
             float4* dst = reinterpret_cast<float4*>(p.part_o + at * DV + c);
 #pragma unroll
             for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
-        if (row_ok) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
+        if (store && g.slot >= 0 && c0 == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
       }
       tc::tc_fence_before();
+      if (!pair) named_bar_sync(2, 256);  // both outputs are read, and the exchange may be written again
     }
   }
   if (!ok && p.status) set_status(p.status, MIMO_ETIMEOUT);
@@ -826,7 +913,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_attn_merge_kernel(cons
         }
       }
     }
-    const float f = sum > 0.f ? 1.f / sum : 0.f;
+    const float f = sum == 0.f ? 0.f : 1.f / sum;
     if (row >= p.T) continue;
     uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + ((size_t)row * p.nq + qh) * DV + lane * VL);
 #pragma unroll
