@@ -81,7 +81,7 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
                                   int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,
                                   int32_t table_width, int32_t page_size, void* plan, size_t plan_bytes,
                                   int32_t* status, void* stream);
-size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads,
                                                 int32_t v_head_dim);
 int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
                              const int32_t* block_table, int32_t table_width, int32_t R, int32_t tokens,

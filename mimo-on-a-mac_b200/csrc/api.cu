@@ -1236,17 +1236,15 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
   p.cu_q = cu_q, p.seq_lens = seq_lens, p.plan = static_cast<int32_t*>(plan), p.status = status;
   p.T = tokens, p.R = R, p.G = n_heads / n_kv_heads, p.nkv = n_kv_heads, p.n = sms, p.width = table_width;
   p.page_shift = page_shift_of(page_size), p.window = window, p.keep = keep_first;
-  p.merge_cost = 1 + paged_attn_part_rows(tokens, p.G) / 64;
   p.key = attn_plan_key(tokens, R, n_heads, n_kv_heads, window, keep_first, table_width, page_size, sms);
   MIMO_TRY(launch_attn_plan(p, static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
 }
 
-size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads,
                                                 int32_t v_head_dim) {
-  if (tokens < 1 || bad_heads(n_heads, n_kv_heads) || v_head_dim < 1) return 0;
-  return (size_t)2 * num_sms_current() * paged_attn_part_rows(tokens, n_heads / n_kv_heads) *
-         ((size_t)v_head_dim + 2) * 4;
+  if (tokens < 1 || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads) || v_head_dim < 1) return 0;
+  return paged_attn_part_rows(tokens, R, n_heads / n_kv_heads, num_sms_current()) * ((size_t)v_head_dim + 2) * 4;
 }
 
 int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const uint16_t* v_pages, const float* sinks,
@@ -1261,7 +1259,7 @@ int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const u
       (int64_t)num_pages * n_kv_heads >= INT32_MAX || bad_table(R, table_width, page_size) || !a16(q) ||
       !a16(k_pages) || !a16(v_pages) || !a16(out) || !a16(plan) || !a16(workspace) ||
       plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads) ||
-      workspace_bytes < mimo_moe_paged_attention_workspace_bytes(tokens, n_heads, n_kv_heads, v_head_dim))
+      workspace_bytes < mimo_moe_paged_attention_workspace_bytes(tokens, R, n_heads, n_kv_heads, v_head_dim))
     return MIMO_EINVAL;
   PagedAttnParams p;
   std::memset(&p, 0, sizeof(p));
@@ -1271,9 +1269,8 @@ int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const u
   p.T = tokens, p.R = R, p.width = table_width, p.nq = n_heads, p.nkv = n_kv_heads, p.G = n_heads / n_kv_heads;
   p.dqk = head_dim, p.dv = v_head_dim, p.window = window, p.keep = keep_first, p.num_pages = num_pages;
   p.page_shift = page_shift_of(page_size), p.scale_log2 = (float)((double)scale * 1.4426950408889634);
-  p.part_rows = paged_attn_part_rows(tokens, p.G);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = p.part_o + (size_t)2 * sms * p.part_rows * v_head_dim;
+  p.part_ml = p.part_o + paged_attn_part_rows(tokens, R, p.G, sms) * v_head_dim;
   p.key = attn_plan_key(tokens, R, n_heads, n_kv_heads, window, keep_first, table_width, page_size, sms);
   MIMO_TRY(launch_paged_attention(p, sms, static_cast<cudaStream_t>(stream)));
   return MIMO_OK;

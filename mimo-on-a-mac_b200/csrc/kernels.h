@@ -349,7 +349,7 @@ struct AttnPlanParams {
   const int32_t *cu_q, *seq_lens;
   int32_t *plan, *status;
   int T, R, G, nkv, n, width, page_shift, window, keep;  // n: CTAs of the attention kernel
-  int merge_cost;                                        // of a split, in key blocks
+  int merge_cost[2];                                     // of a split, in key blocks, for each list of units
   int key;                                               // what the plan was made for
 };
 struct PagedAttnParams {
@@ -358,14 +358,15 @@ struct PagedAttnParams {
   const float* sinks;            // [nq] sink logits, or null
   const int32_t *table, *plan;
   uint16_t* out;                 // [T][nq][dv]
-  float *part_o, *part_ml;       // [2 n][part_rows][dv] unnormalised parts, [2 n][part_rows][2] (max in log2, sum)
+  float *part_o, *part_ml;       // [rows][dv] unnormalised parts, [rows][2] their maximum (log2) and sum
   int32_t* status;
-  int T, R, width, nq, nkv, G, dqk, dv, window, keep, num_pages, page_shift, part_rows, key;
+  int T, R, width, nq, nkv, G, dqk, dv, window, keep, num_pages, page_shift, key;
+  int second;                    // the call's second attention kernel
   float scale_log2;              // softmax scale * log2(e)
 };
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms);
-int paged_attn_part_rows(int T, int G);  // query rows of the largest work unit
-cudaError_t launch_attn_plan(const AttnPlanParams& p, cudaStream_t st);
+size_t paged_attn_part_rows(int T, int R, int G, int num_sms);  // rows of parts a call may write
+cudaError_t launch_attn_plan(AttnPlanParams& p, cudaStream_t st);
 cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st);
 cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st);
 cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st);

@@ -15,9 +15,10 @@
 //                    over S_j's own TMEM columns, where the P V product reads it as its A operand (it never passes
 //                    through shared memory), the row sum from the float32 P.  The output in TMEM is rescaled only
 //                    when a row's maximum grows by more than 2^8 (P stays below 256);
-//   warp 8           TMA producer: Q of both tiles, then K_j and V_j as chunks of 64 dims x 128 positions (16 KB) through
-//                    one ring of shared-memory slots; lane i copies the i-th page of the block (a box of 64 dims x
-//                    page_size positions), and pages nobody sees are read as zeros from behind the pool's end;
+//   warps 8, 11      TMA producers of Q and K, and of V: chunks of 64 dims x 128 positions (16 KB) through one ring of
+//                    shared-memory slots, K_0 V_0 K_1 V_1 ...; lane i copies the i-th page of the block (a box of 64
+//                    dims x page_size positions), and pages nobody sees are read as zeros from behind the pool's end.
+//                    Two warps, because with pages of 16 tokens a block is 40 boxes of about 100 cycles to issue;
 //   warp 9           MMA issuer (one thread): S = Q K^T and O += P V, alternating the tiles, so that one tile's products
 //                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV and its
 //                    next S are issued in this order, so when that S is there, O holds PV and P is consumed;
@@ -40,19 +41,37 @@ constexpr int kThreads = 384;
 constexpr int kRegsSoftmax = 200, kRegsOther = 104;
 
 // ------------------------------------------------------------------------------------------------------------ the plan
-// Layout of the plan buffer (32-bit words, every part 16-byte aligned).
+// There are two lists of work units: small ones (at most kSmallRows query rows) and others, each for a kernel of its own
+// (see Shape).  A request of at most tok[kSmall] new tokens is a small unit; when there are no more rows than requests,
+// all units are small (a request of more tokens is then several).
+constexpr int kSmall = 0, kLarge = 1, kSmallRows = 32;
+
+struct Lists {
+  int tok[2];      // new tokens of a unit at most; 0: the list has none
+  bool all_small;
+};
+__host__ __device__ inline Lists lists_of(int T, int R, int G) {
+  Lists l;
+  l.tok[kSmall] = kSmallRows / G;
+  l.all_small = l.tok[kSmall] > 0 && T <= R;
+  l.tok[kLarge] = l.all_small ? 0 : 2 * (128 / G);
+  return l;
+}
+
+// Layout of one list in the plan buffer (32-bit words from its start, every part 16-byte aligned).
 struct PlanLayout {
-  int n, cap_tiles, cap_segs;
+  int cap_tiles, cap_segs;
   size_t base, count, merge, segs, tiles, nb, order, pre, words;
 };
 
 __host__ __device__ inline size_t up4(size_t x) { return (x + 3) & ~(size_t)3; }
 
-__host__ __device__ inline PlanLayout plan_layout(int T, int R, int G, int nkv, int n) {
+__host__ __device__ inline PlanLayout plan_layout(int list, int T, int R, int G, int nkv, int n) {
   PlanLayout L;
-  const int tok = 2 * (128 / G);
-  L.n = n;
-  L.cap_tiles = R + T / tok;  // sum of ceil(n_r / tok)
+  const Lists ls = lists_of(T, R, G);
+  const int tok = ls.tok[list];
+  // sum of ceil(n_r / tok) over the requests of the list
+  L.cap_tiles = tok == 0 ? 0 : list == kSmall && !ls.all_small ? R : R + T / tok;
   L.cap_segs = L.cap_tiles * nkv + n;
   size_t at = 16;  // header: key, units, mode
   L.base = at, at += up4(n);
@@ -65,6 +84,17 @@ __host__ __device__ inline PlanLayout plan_layout(int T, int R, int G, int nkv, 
   L.pre = at, at += up4((size_t)2 * L.cap_tiles + 2);
   L.words = at;
   return L;
+}
+__host__ __device__ inline size_t list_start(int list, int T, int R, int G, int nkv, int n) {
+  return list == kSmall ? 0 : plan_layout(kSmall, T, R, G, nkv, n).words;
+}
+// Rows of a list's largest unit: one part's rows in the workspace, and the workspace rows before the list's own.
+__host__ __device__ inline int part_rows_of(int list, int T, int R, int G) {
+  const int tok = lists_of(T, R, G).tok[list];
+  return (tok < T ? tok : T) * G;
+}
+__host__ __device__ inline size_t part_start(int list, int T, int R, int G, int n) {
+  return list == kSmall ? 0 : (size_t)2 * n * part_rows_of(kSmall, T, R, G);
 }
 
 // Key blocks of a unit whose queries are at qfirst .. qlast.
@@ -108,7 +138,7 @@ __device__ __forceinline__ long long block_scan(long long v, long long* excl, lo
   return tot;
 }
 
-// One CTA.  Two ways to deal the units to the n CTAs: whole units, longest first, in a snake (no partial results), or
+// One CTA for each list.  Two ways to deal the units to the n CTAs: whole units, longest first, in a snake (no partial results), or
 // the units' blocks one after another in n equal ranges (perfect balance; a unit cut by a range's end leaves partial
 // results that the merge kernel joins).  The one whose longest CTA takes less is taken, in units of a key block, each
 // unit counted as its blocks and kUnitCost more.
@@ -120,15 +150,18 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
   __shared__ long long sh[kPlanThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x, n = p.n;
-  const int tok = 2 * (128 / p.G);
-  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, n);
-  int4* tiles = reinterpret_cast<int4*>(p.plan + L.tiles);
-  int* nbs = p.plan + L.nb;
-  int* order = p.plan + L.order;
-  long long* pre = reinterpret_cast<long long*>(p.plan + L.pre);
-  int4* segs = reinterpret_cast<int4*>(p.plan + L.segs);
-  int4* merge = reinterpret_cast<int4*>(p.plan + L.merge);
+  const int tid = threadIdx.x, n = p.n, list = blockIdx.x;
+  const Lists ls = lists_of(p.T, p.R, p.G);
+  const int tok = ls.tok[list];
+  if (tok == 0) return;
+  const PlanLayout L = plan_layout(list, p.T, p.R, p.G, p.nkv, n);
+  int32_t* plan = p.plan + list_start(list, p.T, p.R, p.G, p.nkv, n);
+  int4* tiles = reinterpret_cast<int4*>(plan + L.tiles);
+  int* nbs = plan + L.nb;
+  int* order = plan + L.order;
+  long long* pre = reinterpret_cast<long long*>(plan + L.pre);
+  int4* segs = reinterpret_cast<int4*>(plan + L.segs);
+  int4* merge = reinterpret_cast<int4*>(plan + L.merge);
   for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   load[tid] = 0;
   // ---- tiles of each request; one whose lengths do not fit has none
@@ -141,10 +174,11 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
         bad = true;
         return 0;
       }
-      return (e - a + tok - 1) / tok;
+      const bool small = ls.all_small || (e - a) <= ls.tok[kSmall];
+      return small == (list == kSmall) ? (e - a + tok - 1) / tok : 0;
     };
-    // the rows of all requests together are at most T, so the tiles fit cap_tiles; a table of overlapping rows could
-    // claim more, and is cut off there
+    // the rows of all requests together are at most T, so the tiles fit cap_tiles; overlapping rows could claim more,
+    // and are cut off there
     long long mine = 0, ex;
     for (int r = r0; r < r1; ++r) mine += count(r);
     const long long tot = block_scan(mine, &ex, sh);
@@ -225,14 +259,14 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
   for (int w = 0; w < kPlanThreads / 32; ++w) most = max(most, load[w]);
   // a CTA's range holds at least two blocks: a shorter one costs more in its partial result than it saves
   const long long quota = max(2ll + kUnitCost, (W + n - 1) / n);
-  const bool split = quota + p.merge_cost < most;
+  const bool split = quota + p.merge_cost[list] < most;
   if (tid == 0) {
-    p.plan[1] = units;
-    p.plan[2] = split ? 1 : 0;
-    p.plan[0] = p.key;
+    plan[1] = units;
+    plan[2] = split ? 1 : 0;
+    plan[0] = p.key;
   }
-  int* base = p.plan + L.base;
-  int* cnt = p.plan + L.count;
+  int* base = plan + L.base;
+  int* cnt = plan + L.count;
   for (int c = tid; c < n; c += kPlanThreads) {
     merge[2 * c] = make_int4(0, 0, 0, 0);
     if (!split) {
@@ -352,28 +386,43 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
+// A box of a 3-D tensor map into shared memory, completing on `bar` (no multicast).
+__device__ __forceinline__ void tma_box(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
+}
+
 constexpr uint32_t kHead = 1024 + 2048;  // barriers, the exchange between the softmax groups; tiles start at a multiple
                                          // of 1024 bytes, as the block's shared memory does
 constexpr uint32_t kChunk = 16384;  // 128 positions x 64 dims, bf16
 
-template <int DQK, int DV>
+// Shared memory of the kernel of each list.  A tile of the MMA is 128 rows either way; a small unit's Q is only
+// kSmallRows of them in memory (the MMA reads what lies behind for the others, and nobody reads their results), which
+// leaves the ring of K and V room for what HBM's latency needs in flight: with the ring that two whole Q tiles leave, a
+// decoding request's block took 2.5 us, most of it the wait for K.
+template <int DQK, int DV, int LIST>
 struct Shape {
   static constexpr int QCH = DQK / 64, VCH = DV / 64;
-  static constexpr uint32_t QB = 128u * DQK * 2;
-  static constexpr int NG = 16;  // barriers of K and V blocks: more than the ring holds (12 chunks at most)
+  static constexpr uint32_t QCHUNK = (LIST == kSmall ? kSmallRows : 128) * 128u;  // 64 dims of a Q tile
+  static constexpr uint32_t QB = QCH * QCHUNK;
+  static constexpr int NG = 16;  // barriers of K and V blocks: more than the ring holds
   static constexpr int NS = (int)((232448u - kHead - 2 * QB) / kChunk);  // ring slots in what Q leaves
   static constexpr uint32_t SMEM = kHead + 2 * QB + NS * kChunk;
   // a single tile's second K block is read before its first V block leaves the ring
   static_assert(2 * QCH + VCH <= NS, "the ring must hold K, V and the next K");
+  static_assert(2 * ((NS + QCH + VCH - 1) / (QCH + VCH)) < NG, "a barrier for every block in the ring");
 };
 
 struct Seg {
   int row0, ntok, qfirst, r, hk, b0, nblk, slot;
 };
 
-template <int DQK, int DV>
+template <int DQK, int DV, int LIST>
 __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
-  using S = Shape<DQK, DV>;
+  using S = Shape<DQK, DV, LIST>;
   constexpr int NS = S::NS, NG = S::NG, CPB = S::QCH + S::VCH;  // ring slots, block barriers, chunks per block
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem);
@@ -419,15 +468,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tbase = *tslot;
-  pdl_wait();  // q, the cache and the plan come from preceding kernels (programmatic dependent launch)
+  // q, the cache and the plan come from preceding kernels (programmatic dependent launch).  Where both lists have a
+  // kernel, the small one comes second and runs beside the large one, which it does not depend on: it may start when
+  // all CTAs of the large one are past this wait, and so are those kernels; it waits for the large one at its end.
+  if (!p.second) pdl_wait();
   pdl_launch_dependents();
 
-  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, gridDim.x);
-  const bool planned = p.plan[0] == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
+  const PlanLayout L = plan_layout(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
+  const int32_t* plan = p.plan + list_start(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
+  const bool planned = plan[0] == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
   if (!planned && threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
-  const int sbase = planned ? p.plan[L.base + blockIdx.x] : 0, nseg = planned ? p.plan[L.count + blockIdx.x] : 0;
-  const int4* segs = reinterpret_cast<const int4*>(p.plan + L.segs) + 2 * (size_t)sbase;
-  const int tpt = 128 / p.G;  // tokens per tile
+  const int sbase = planned ? plan[L.base + blockIdx.x] : 0, nseg = planned ? plan[L.count + blockIdx.x] : 0;
+  const int4* segs = reinterpret_cast<const int4*>(plan + L.segs) + 2 * (size_t)sbase;
+  const int tpt = (LIST == kSmall ? kSmallRows : 128) / p.G;  // tokens per tile
+  const int part_rows = part_rows_of(LIST, p.T, p.R, p.G);
+  const size_t part0 = part_start(LIST, p.T, p.R, p.G, gridDim.x);
   auto load_seg = [&](int s) -> Seg {
     const int4 a = segs[2 * s], b = segs[2 * s + 1];
     return Seg{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -436,16 +491,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
-    if (warp == 8) {  // ------------------------------------------------------------------------- TMA producer
+    if (warp == 8 || warp == 11) {  // ------------------------------------------------- TMA producers: Q and K, V
+      const bool isv = warp == 11;
+      const CUtensorMap* map = isv ? &p.vmap : &p.kmap;
+      const int chunks = isv ? S::VCH : S::QCH;
       if (lane == 0) {
-        tma_prefetch_map(&p.qmap);
-        tma_prefetch_map(&p.kmap);
-        tma_prefetch_map(&p.vmap);
+        tma_prefetch_map(map);
+        if (!isv) tma_prefetch_map(&p.qmap);
       }
-      const uint64_t pol = tc::l2_evict_normal_policy();
       const int P = 1 << p.page_shift, ppb = 128 >> p.page_shift;  // pages per block
       const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
-      uint32_t ci = 0, nb = 0;                                     // chunks and key blocks issued
+      uint32_t ci = isv ? S::QCH : 0, nb = 0;                      // ring chunk, key blocks issued
       uint32_t freed = 0;                                          // ring blocks known to be free again
       uint32_t nq = 0, turn = 0;                                   // phases of the Q buffers, the next single tile's
       for (int s = 0; s < nseg && ok; ++s) {
@@ -468,60 +524,50 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         int row = page_of(g.b0);
         for (int j = 0; j < g.nblk && ok; ++j) {
           const int next = j + 1 < g.nblk ? page_of(g.b0 + j + 1) : 0;
-#pragma unroll
-          for (int c = 0; c < CPB; ++c) {
-            if (c == S::QCH && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
-              const bool pair = g.ntok > tpt;
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int qb = pair ? x : turn;
-                if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
-                nq ^= 1u << qb;
-                if (lane == 0 && ok) {
-                  mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
-#pragma unroll
-                  for (int d = 0; d < S::QCH; ++d)
-                    tma_load_3d(sQ + qb * S::QB + d * kChunk, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt,
-                                &q_full[qb], pol);
-                }
-                if (!pair) break;
-              }
-              if (!pair) turn ^= 1;
-            }
-            if (ci >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
-              const uint32_t old = ci - NS, g = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
-              if (ok && g >= freed) ok = mbar_wait(&empty[g % NG], (g / NG) & 1);
-              freed = g + 1;
+          uint64_t* bar = &full[(2 * nb + (isv ? 1 : 0)) % NG];
+          for (int c = 0; c < chunks; ++c) {
+            if (ci + c >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
+              const uint32_t old = ci + c - NS, of = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
+              if (ok && of >= freed) ok = mbar_wait(&empty[of % NG], (of / NG) & 1);
+              freed = of + 1;
             }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
-            const uint32_t sl = ci % NS;
-            uint64_t* bar = &full[(2 * nb + (c >= S::QCH ? 1 : 0)) % NG];
-            if (c == 0 || c == S::QCH) {
-              if (lane == 0) mbar_arrive_expect_tx(bar, (c == 0 ? S::QCH : S::VCH) * kChunk);
+            if (c == 0) {
+              if (lane == 0) mbar_arrive_expect_tx(bar, chunks * kChunk);
               __syncwarp();
             }
-            if (lane < ppb) {
-              uint8_t* dst = sRing + sl * kChunk + (uint32_t)lane * P * 128;
-              if (c < S::QCH)
-                tma_load_3d(dst, &p.kmap, c * 64, 0, row, bar, pol);
-              else
-                tma_load_3d(dst, &p.vmap, (c - S::QCH) * 64, 0, row, bar, pol);
-            }
-            ++ci;
+            if (lane < ppb)
+              tma_box(sRing + ((ci + c) % NS) * kChunk + (uint32_t)lane * P * 128, map, c * 64, 0, row, bar);
           }
+          if (!isv && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
+            const bool pair = LIST == kLarge && g.ntok > tpt;
+            for (int x = 0; x < (pair ? 2 : 1); ++x) {
+              const int qb = pair ? x : turn;
+              if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
+              nq ^= 1u << qb;
+              if (lane == 0 && ok) {
+                mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
+#pragma unroll
+                for (int d = 0; d < S::QCH; ++d)
+                  tma_box(sQ + qb * S::QB + d * S::QCHUNK, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[qb]);
+              }
+            }
+            if (!pair) turn ^= 1;
+          }
+          ci += CPB;
           ++nb;
           row = next;
         }
       }
       // no copy may still be landing when the CTA exits: the last blocks (after a wait that ran out, what there is of
-      // the block it was in: these waits run out too), and Q
-      if (!ok) mbar_wait(&full[(2 * nb) % NG], (2 * nb / NG) & 1), mbar_wait(&full[(2 * nb + 1) % NG], ((2 * nb + 1) / NG) & 1);
-      for (uint32_t k = 0; k < (uint32_t)NG && k < 2 * nb; ++k) {
-        const uint32_t i = 2 * nb - 1 - k;
+      // the block it was in: this wait runs out too), and Q
+      for (uint32_t k = 0; k < (uint32_t)NG / 2 && k < nb; ++k) {
+        const uint32_t i = 2 * (nb - 1 - k) + (isv ? 1 : 0);
         mbar_wait(&full[i % NG], (i / NG) & 1);
       }
-      for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
+      if (!isv)
+        for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
     } else if (warp == 9) {
       if (lane == 0) {  // ------------------------------------------------------------------------- MMA issuer
         const uint32_t idesc_s = tc::idesc_bf16(128, 128);
@@ -553,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           const uint32_t d = tbase + x * 128;
 #pragma unroll
           for (int c = 0; c < S::QCH; ++c) {
-            const uint32_t a = aq + (qb * S::QB + c * kChunk) / 16, b = bk + wrap(at + c) * (kChunk / 16);
+            const uint32_t a = aq + (qb * S::QB + c * S::QCHUNK) / 16, b = bk + wrap(at + c) * (kChunk / 16);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) mma_ss(d, a + kk * 2, b + kk * 2, idesc_s, (c | kk) != 0);
           }
@@ -584,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb), kp = kb * 128;
             return !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
           };
-          if (g.ntok > tpt) {  // a pair: both tiles on every block
+          if (LIST == kLarge && g.ntok > tpt) {  // a pair: both tiles on every block
             there(2 * nb);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
@@ -696,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     uint32_t ns = 0, no = 0;
     for (int s = 0; s < nseg; ++s) {
       const Seg g = load_seg(s);
-      const bool pair = g.ntok > tpt;
+      const bool pair = LIST == kLarge && g.ntok > tpt;
       const int tt = r / p.G + (pair ? x * tpt : 0);  // its token of the unit
       const Blocks bl = blocks_of(g.qfirst, g.qfirst + g.ntok - 1, p.window, p.keep);
       const bool row_ok = r < tpt * p.G && tt < g.ntok;
@@ -819,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         }
         w_own *= f, w_other *= f;
         const bool store = row_ok && row < p.T;
-        const size_t at = (size_t)max(g.slot, 0) * p.part_rows + (tt * p.G + head);
+        const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
 #pragma unroll 1
         for (int c = c0; c < c1; c += 32) {
           float o[32];
@@ -862,6 +908,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     tc::tc_fence_after();
     tc::tmem_dealloc(tbase, 512);
   }
+  if (p.second) pdl_wait();
 }
 
 // ------------------------------------------------------------------------------------------------------------ merge
@@ -874,14 +921,18 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_attn_merge_kernel(cons
   constexpr int VL = DV / 32;
   pdl_wait();
   pdl_launch_dependents();
-  const PlanLayout L = plan_layout(p.T, p.R, p.G, p.nkv, gridDim.x);
-  if (p.plan[0] != p.key) return;
-  const int4* mg = reinterpret_cast<const int4*>(p.plan + L.merge) + 2 * (size_t)blockIdx.x;
+  const int list = lists_of(p.T, p.R, p.G).tok[blockIdx.z] > 0 ? blockIdx.z : 1 - blockIdx.z;
+  const PlanLayout L = plan_layout(list, p.T, p.R, p.G, p.nkv, gridDim.x);
+  const int32_t* plan = p.plan + list_start(list, p.T, p.R, p.G, p.nkv, gridDim.x);
+  if (plan[0] != p.key) return;
+  const int part_rows = part_rows_of(list, p.T, p.R, p.G);
+  const size_t part0 = part_start(list, p.T, p.R, p.G, gridDim.x);
+  const int4* mg = reinterpret_cast<const int4*>(plan + L.merge) + 2 * (size_t)blockIdx.x;
   const int4 a = mg[0], b = mg[1];  // row0, tokens, kv head, first CTA; slot of the first part, parts
   const int lane = threadIdx.x & 31;
   for (int rr = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); rr < a.y * p.G; rr += gridDim.y * kMergeWarps) {
     const int tt = rr / p.G, qh = a.z * p.G + rr % p.G, row = a.x + tt;
-    auto part = [&](int s) -> size_t { return (size_t)(s == 0 ? b.x : 2 * (a.w + s)) * p.part_rows + rr; };
+    auto part = [&](int s) -> size_t { return part0 + (size_t)(s == 0 ? b.x : 2 * (a.w + s)) * part_rows + rr; };
     const float sink = p.sinks ? p.sinks[qh] * kLog2e : -INFINITY;
     float M = sink;
     for (int s = lane; s < b.y; s += 32) M = fmaxf(M, p.part_ml[part(s) * 2]);
@@ -921,41 +972,60 @@ __global__ void __launch_bounds__(kMergeWarps * 32) paged_attn_merge_kernel(cons
   }
 }
 
-template <int DQK, int DV>
-cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
-  using S = Shape<DQK, DV>;
+template <int DQK, int DV, int LIST>
+cudaError_t launch_list(PagedAttnParams& p, int num_sms, cudaStream_t st) {
+  using S = Shape<DQK, DV, LIST>;
   static bool attr_set[128] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 128 && !attr_set[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<DQK, DV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               (int)S::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(paged_attn_kernel<DQK, DV, LIST>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  const cudaError_t e = launch_k(paged_attn_kernel<DQK, DV>, dim3(num_sms), dim3(kThreads), S::SMEM, st, p);
+  const int tile = (LIST == kSmall ? kSmallRows : 128) / p.G;  // tokens
+  const cudaError_t e = bf16_map3(&p.qmap, p.q, (uint64_t)DQK, (uint64_t)p.nq, (uint64_t)p.T, p.G, tile);
   if (e != cudaSuccess) return e;
-  return launch_k(paged_attn_merge_kernel<DV>, dim3(num_sms, std::min(4, (p.part_rows + kMergeWarps - 1) / kMergeWarps)),
+  return launch_k(paged_attn_kernel<DQK, DV, LIST>, dim3(num_sms), dim3(kThreads), S::SMEM, st, p);
+}
+
+template <int DQK, int DV>
+cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
+  const Lists ls = lists_of(p.T, p.R, p.G);
+  const bool both = ls.tok[kSmall] > 0 && ls.tok[kLarge] > 0;
+  cudaError_t e = cudaSuccess;
+  if (ls.tok[kLarge] > 0) e = launch_list<DQK, DV, kLarge>(p, num_sms, st);
+  if (e != cudaSuccess) return e;
+  p.second = both ? 1 : 0;
+  if (ls.tok[kSmall] > 0) e = launch_list<DQK, DV, kSmall>(p, num_sms, st);
+  if (e != cudaSuccess) return e;
+  const int rows = std::max(part_rows_of(kSmall, p.T, p.R, p.G), part_rows_of(kLarge, p.T, p.R, p.G));
+  return launch_k(paged_attn_merge_kernel<DV>,
+                  dim3(num_sms, std::min(4, (rows + kMergeWarps - 1) / kMergeWarps), both ? 2 : 1),
                   dim3(kMergeWarps * 32), 0, st, p);
 }
 
 }  // namespace
 
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms) {
-  return plan_layout(T, R, G, nkv, num_sms).words * 4;
+  return 4 * (list_start(kLarge, T, R, G, nkv, num_sms) + plan_layout(kLarge, T, R, G, nkv, num_sms).words);
 }
 
-int paged_attn_part_rows(int T, int G) { return std::min(2 * (128 / G), T) * G; }
+size_t paged_attn_part_rows(int T, int R, int G, int num_sms) {
+  return part_start(kLarge, T, R, G, num_sms) + (size_t)2 * num_sms * part_rows_of(kLarge, T, R, G);
+}
 
-cudaError_t launch_attn_plan(const AttnPlanParams& p, cudaStream_t st) {
-  return launch_k(attn_plan_kernel, dim3(1), dim3(kPlanThreads), (size_t)(p.R + 1) * 4, st, p);
+cudaError_t launch_attn_plan(AttnPlanParams& p, cudaStream_t st) {
+  // a split's cost in blocks: its parts' rows written and read again, and the merge
+  for (int l : {kSmall, kLarge}) p.merge_cost[l] = 1 + part_rows_of(l, p.T, p.R, p.G) / 64;
+  return launch_k(attn_plan_kernel, dim3(2), dim3(kPlanThreads), (size_t)(p.R + 1) * 4, st, p);
 }
 
 cudaError_t launch_paged_attention(PagedAttnParams& p, int num_sms, cudaStream_t st) {
   const uint64_t rows = (uint64_t)p.num_pages * p.nkv;
   const int P = 1 << p.page_shift;
-  cudaError_t e = bf16_map3(&p.qmap, p.q, (uint64_t)p.dqk, (uint64_t)p.nq, (uint64_t)p.T, p.G, 128 / p.G);
-  if (e == cudaSuccess) e = bf16_map3(&p.kmap, p.k, (uint64_t)p.dqk, (uint64_t)P, rows, P, 1);
+  cudaError_t e = bf16_map3(&p.kmap, p.k, (uint64_t)p.dqk, (uint64_t)P, rows, P, 1);
   if (e == cudaSuccess) e = bf16_map3(&p.vmap, p.v, (uint64_t)p.dv, (uint64_t)P, rows, P, 1);
   if (e != cudaSuccess) return e;
   if (p.dqk == 192) return launch_t<192, 128>(p, num_sms, st);

@@ -109,7 +109,7 @@ SIGNATURES = {
     "mimo_moe_paged_attention_plan_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "mimo_moe_paged_attention_plan": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                                 c_int32, c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "mimo_moe_paged_attention_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
+    "mimo_moe_paged_attention_workspace_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "mimo_moe_paged_attention": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32,
                                            c_int32, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_int32,
                                            c_int32, c_void_p, c_size_t, c_void_p, c_void_p, c_size_t, c_void_p,

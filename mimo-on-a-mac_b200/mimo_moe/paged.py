@@ -352,7 +352,8 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
         return o
     with _on(dev):
         L = lib()
-        nb = L.mimo_moe_paged_attention_workspace_bytes(T, cfg.n_heads, cfg.n_kv_heads, cfg.v_head_dim)
+        nb = L.mimo_moe_paged_attention_workspace_bytes(T, step.requests, cfg.n_heads, cfg.n_kv_heads,
+                                                         cfg.v_head_dim)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev)   # the call's own: two streams or graphs never share it
         check(L.mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
                                          step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,

@@ -87,7 +87,7 @@ def test_paged_attention_refuses(bad):
              keep=4, pages=8, P=16, plan=A, nb=0, out=A, ws=A, wb=0, status=None, stream=None)
     d.update({k: v for k, v in bad.items() if k not in ("nb", "wb")})
     d["nb"] = max(0, L.mimo_moe_paged_attention_plan_bytes(40, 2, 8, 2)) + 10**9 - 10**9 * (("nb" in bad) or 0)
-    d["wb"] = 10**10 if "wb" not in bad else L.mimo_moe_paged_attention_workspace_bytes(40, 8, 2, 128) - 1
+    d["wb"] = 10**10 if "wb" not in bad else L.mimo_moe_paged_attention_workspace_bytes(40, 2, 8, 2, 128) - 1
     if "nb" in bad:
         d["nb"] -= 1
     assert L.mimo_moe_paged_attention(*d.values()) == EINVAL
