@@ -16,10 +16,10 @@
 //                    through shared memory), the row sum from the float32 P.  The output in TMEM is rescaled only
 //                    when a row's maximum grows by more than 2^8 (P stays below 256);
 //   warps 8, 11      TMA producers of Q and K, and of V: chunks of 64 dims x 128 positions (16 KB) through one ring of
-//                    shared-memory slots, K_0 V_0 K_1 V_1 ...; lane i copies the i-th page of the block (a box of 64
-//                    dims x page_size positions), and pages nobody sees are read as zeros from behind the pool's end.
-//                    Two warps, because with pages of 16 tokens a block is 40 boxes of about 100 cycles to issue;
-//   warp 9           MMA issuer (one thread): S = Q K^T and O += P V, alternating the tiles, so that one tile's products
+//                    shared-memory slots, K_0 V_0 K_1 V_1 ...; a box is
+//                    64 dims of a page, and pages nobody sees are read as zeros from behind the pool's end.  Two warps,
+//                    because with pages of 16 tokens a block is 40 boxes;
+//   warp 9           MMA issuer: S = Q K^T and O += P V, alternating the tiles, so that one tile's products
 //                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV and its
 //                    next S are issued in this order, so when that S is there, O holds PV and P is consumed;
 //   warp 10          zeroes the V rows that no query of the unit sees in the blocks at the range's ends: such slots may
@@ -61,7 +61,7 @@ __host__ __device__ inline Lists lists_of(int T, int R, int G) {
 // Layout of one list in the plan buffer (32-bit words from its start, every part 16-byte aligned).
 struct PlanLayout {
   int cap_tiles, cap_segs;
-  size_t base, count, merge, segs, tiles, nb, order, pre, words;
+  size_t head, merge, segs, tiles, nb, order, pre, words;
 };
 
 __host__ __device__ inline size_t up4(size_t x) { return (x + 3) & ~(size_t)3; }
@@ -74,8 +74,7 @@ __host__ __device__ inline PlanLayout plan_layout(int list, int T, int R, int G,
   L.cap_tiles = tok == 0 ? 0 : list == kSmall && !ls.all_small ? R : R + T / tok;
   L.cap_segs = L.cap_tiles * nkv + n;
   size_t at = 16;  // header: key, units, mode
-  L.base = at, at += up4(n);
-  L.count = at, at += up4(n);
+  L.head = at, at += (size_t)12 * n;  // of each CTA: (its first segment's place, segments), the first segment itself
   L.merge = at, at += (size_t)8 * n;
   L.segs = at, at += (size_t)8 * L.cap_segs;
   L.tiles = at, at += (size_t)4 * L.cap_tiles;
@@ -162,6 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
   long long* pre = reinterpret_cast<long long*>(plan + L.pre);
   int4* segs = reinterpret_cast<int4*>(plan + L.segs);
   int4* merge = reinterpret_cast<int4*>(plan + L.merge);
+  int4* head = reinterpret_cast<int4*>(plan + L.head);
   for (int i = tid; i < kBuckets; i += kPlanThreads) hist[i] = 0;
   load[tid] = 0;
   // ---- tiles of each request; one whose lengths do not fit has none
@@ -265,16 +265,13 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     plan[2] = split ? 1 : 0;
     plan[0] = p.key;
   }
-  int* base = plan + L.base;
-  int* cnt = plan + L.count;
   for (int c = tid; c < n; c += kPlanThreads) {
     merge[2 * c] = make_int4(0, 0, 0, 0);
     if (!split) {
       const int full = units / n, rest = units % n;
-      base[c] = c * K;
-      cnt[c] = full + (((full & 1) ? n - 1 - c : c) < rest ? 1 : 0);
+      head[3 * c] = make_int4(c * K, full + (((full & 1) ? n - 1 - c : c) < rest ? 1 : 0), 0, 0);
     } else if (c * quota >= W) {
-      base[c] = 0, cnt[c] = 0;
+      head[3 * c] = make_int4(0, 0, 0, 0);
     } else {
       // the unit that holds x on the line of all units' costs, and where its first block lies (its own cost comes before)
       long long first_block;
@@ -291,17 +288,17 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
       const long long end = min(W, (c + 1) * quota);
       const int first = unit_at(c * quota) + (first_block >= end ? 1 : 0);
       const int last = unit_at(end - 1) - (first_block >= end ? 1 : 0);
-      base[c] = first + c;
-      cnt[c] = max(0, last - first + 1);
+      head[3 * c] = make_int4(first + c, max(0, last - first + 1), 0, 0);
     }
   }
   __syncthreads();
   for (int u = tid; u < units; u += kPlanThreads) {
     if (!split) {
       const int i = order[u / p.nkv], c = cta_of(u);
+      const int4 a = tiles[i], b = make_int4(u % p.nkv, 0, nbs[i], -1);
       int4* s = segs + 2 * ((size_t)c * K + u / n);
-      s[0] = tiles[i];
-      s[1] = make_int4(u % p.nkv, 0, nbs[i], -1);
+      s[0] = a, s[1] = b;
+      if (u < n) head[3 * c + 1] = a, head[3 * c + 2] = b;
     } else {
       const int i = u / p.nkv, hk = u % p.nkv, nb = nbs[i];
       const int4 t = tiles[i];
@@ -310,11 +307,13 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
       int slot0 = -1;
       for (int c = c0; c <= c1; ++c) {
         const int b0 = (int)(max(s0, c * quota) - s0), b1 = (int)(min(s1, (c + 1) * quota) - s0);
-        const int slot = c0 == c1 ? -1 : 2 * c + (base[c] == u + c ? 0 : 1);  // a CTA's first segment, or its last
+        const bool first = head[3 * c].x == u + c;
+        const int slot = c0 == c1 ? -1 : 2 * c + (first ? 0 : 1);  // a CTA's first segment, or its last
         if (c == c0) slot0 = slot;
+        const int4 b = make_int4(hk, b0, b1 - b0, slot);
         int4* s = segs + 2 * ((size_t)u + c);
-        s[0] = t;
-        s[1] = make_int4(hk, b0, b1 - b0, slot);
+        s[0] = t, s[1] = b;
+        if (first) head[3 * c + 1] = t, head[3 * c + 2] = b;
       }
       if (c1 > c0) {  // at most one unit runs over the end of CTA c0's range
         merge[2 * c0] = make_int4(t.x, t.y, hk, c0);
@@ -334,6 +333,35 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rn(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+// Two float32 operations in one instruction, each rounded as its scalar form.
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
 }
 // 32 TMEM columns of the warp's 32 lanes
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
@@ -386,6 +414,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
+// True in one lane of the warp, which must be whole here.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n.reg .pred q;\nelect.sync _|q, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, q;\n}\n" : "=r"(r));
+  return r != 0;
+}
 // A box of a 3-D tensor map into shared memory, completing on `bar` (no multicast).
 __device__ __forceinline__ void tma_box(void* dst, const void* map, int c0, int c1, int c2, uint64_t* bar) {
   asm volatile(
@@ -476,17 +510,28 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 
   const PlanLayout L = plan_layout(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
   const int32_t* plan = p.plan + list_start(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
-  const bool planned = plan[0] == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
+  const int key = plan[0];
+  const int4* head = reinterpret_cast<const int4*>(plan + L.head) + 3 * blockIdx.x;
+  const int4 where = head[0], first_a = head[1], first_b = head[2];
+  const bool planned = key == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
   if (!planned && threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
-  const int sbase = planned ? plan[L.base + blockIdx.x] : 0, nseg = planned ? plan[L.count + blockIdx.x] : 0;
-  const int4* segs = reinterpret_cast<const int4*>(plan + L.segs) + 2 * (size_t)sbase;
+  const int nseg = planned ? where.y : 0;
+  const int4* segs = reinterpret_cast<const int4*>(plan + L.segs) + 2 * (size_t)where.x;
   const int tpt = (LIST == kSmall ? kSmallRows : 128) / p.G;  // tokens per tile
   const int part_rows = part_rows_of(LIST, p.T, p.R, p.G);
   const size_t part0 = part_start(LIST, p.T, p.R, p.G, gridDim.x);
-  auto load_seg = [&](int s) -> Seg {
-    const int4 a = segs[2 * s], b = segs[2 * s + 1];
-    return Seg{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  };
+  // the CTA's segments in turn, the next one's load in flight while one is worked on
+  struct Segs {
+    const int4* at;
+    int4 a, b;
+    int left;
+    __device__ __forceinline__ Seg next() {
+      const Seg g{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      at += 2;
+      if (--left > 0) a = at[0], b = at[1];
+      return g;
+    }
+  } list{segs, first_a, first_b, nseg};
   bool ok = true;
 
   if (warp >= 8) {
@@ -505,25 +550,26 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       uint32_t freed = 0;                                          // ring blocks known to be free again
       uint32_t nq = 0, turn = 0;                                   // phases of the Q buffers, the next single tile's
       for (int s = 0; s < nseg && ok; ++s) {
-        const Seg g = load_seg(s);
+        const Seg g = list.next();
         const int qlast = g.qfirst + g.ntok - 1;
         const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
         const int* trow = p.table + (size_t)g.r * p.width;
-        // the page (its row in the maps) that this lane copies of block j
+        // the number of the block's page `lane`, num_pages for one nobody sees; loaded a block ahead
         auto page_of = [&](int j) -> int {
           const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb);
           const int pg = kb * ppb + lane, pos = pg << p.page_shift;
-          if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return nowhere;
-          const int id = trow[pg];
-          if ((unsigned)id >= (unsigned)p.num_pages) {
-            set_status(p.status, MIMO_ERANGE);
-            return nowhere;
-          }
-          return id * p.nkv + g.hk;
+          if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return p.num_pages;
+          return trow[pg];
         };
-        int row = page_of(g.b0);
+        int page = page_of(g.b0);
         for (int j = 0; j < g.nblk && ok; ++j) {
-          const int next = j + 1 < g.nblk ? page_of(g.b0 + j + 1) : 0;
+          int row = nowhere;
+          if ((unsigned)page < (unsigned)p.num_pages) row = page * p.nkv + g.hk;
+          else if (page != p.num_pages) set_status(p.status, MIMO_ERANGE);
+          if (j + 1 < g.nblk) page = page_of(g.b0 + j + 1);
+          int rows[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, row, i);
           uint64_t* bar = &full[(2 * nb + (isv ? 1 : 0)) % NG];
           for (int c = 0; c < chunks; ++c) {
             if (ci + c >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
@@ -533,12 +579,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             }
             ok = __all_sync(0xFFFFFFFFu, ok);
             if (!ok) break;
-            if (c == 0) {
-              if (lane == 0) mbar_arrive_expect_tx(bar, chunks * kChunk);
-              __syncwarp();
+            if (lane == 0) {
+              if (c == 0) mbar_arrive_expect_tx(bar, chunks * kChunk);
+              uint8_t* dst = sRing + ((ci + c) % NS) * kChunk;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                if (i < ppb) tma_box(dst + i * P * 128, map, c * 64, 0, rows[i], bar);
             }
-            if (lane < ppb)
-              tma_box(sRing + ((ci + c) % NS) * kChunk + (uint32_t)lane * P * 128, map, c * 64, 0, row, bar);
+            __syncwarp();
           }
           if (!isv && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
             const bool pair = LIST == kLarge && g.ntok > tpt;
@@ -557,7 +605,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           }
           ci += CPB;
           ++nb;
-          row = next;
         }
       }
       // no copy may still be landing when the CTA exits: the last blocks (after a wait that ran out, what there is of
@@ -569,34 +616,39 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       if (!isv)
         for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
     } else if (warp == 9) {
-      if (lane == 0) {  // ------------------------------------------------------------------------- MMA issuer
-        const uint32_t idesc_s = tc::idesc_bf16(128, 128);
-        const uint32_t idesc_o64 = tc::idesc_bf16(128, 64) | (1u << 16);  // B = V, MN-major
-        const uint32_t idesc_o = tc::idesc_bf16(128, DV) | (1u << 16);
-        const uint32_t aq = desc_k(smem_u32(sQ)), bk = desc_k(smem_u32(sRing)), bv = desc_mn(smem_u32(sRing));
-        uint32_t nb = 0, slot = 0;  // key blocks before this one, ring slot of its first chunk
-        uint32_t nq = 0, turn = 0, np = 0, nfix = 0;  // phases
-        auto there = [&](uint32_t g) {
-          if (ok) ok = mbar_wait(&full[g % NG], (g / NG) & 1);
-          tc::tc_fence_after();
-        };
-        auto wrap = [](uint32_t sl) -> uint32_t { return sl >= (uint32_t)NS ? sl - NS : sl; };
-        auto q_there = [&](int qb) {
-          if (ok) ok = mbar_wait(&q_full[qb], (nq >> qb) & 1);
-          nq ^= 1u << qb;
-          tc::tc_fence_after();
-        };
-        auto p_there = [&](int x) {
-          if (ok) ok = mbar_wait(&p_full[x], (np >> x) & 1);
-          np ^= 1u << x;
-        };
-        auto fixed = [&]() {
-          if (ok) ok = mbar_wait(v_fixed, nfix & 1);
-          ++nfix;
-        };
-        // S = Q K^T of tile x from Q buffer qb and the K chunks at ring slot `at`
-        auto issue_s = [&](int x, int qb, uint32_t at) {
-          const uint32_t d = tbase + x * 128;
+      // --------------------------------------------------------------------------------------------- MMA issuer
+      // The whole warp runs this and one elected lane issues: what all lanes agree on stays in uniform registers, which
+      // the MMA reads its operands from.  (From a branch of one lane an MMA took 70 cycles to issue, 90 to 100 beside
+      // the softmax warps; this way 64, the tensor core's own time for 128 x 128 x 16.)
+      const uint32_t idesc_s = tc::idesc_bf16(128, 128);
+      const uint32_t idesc_o64 = tc::idesc_bf16(128, 64) | (1u << 16);  // B = V, MN-major
+      const uint32_t idesc_o = tc::idesc_bf16(128, DV) | (1u << 16);
+      const uint32_t aq = desc_k(smem_u32(sQ)), bk = desc_k(smem_u32(sRing)), bv = desc_mn(smem_u32(sRing));
+      const uint32_t tb = __shfl_sync(0xFFFFFFFFu, tbase, 0);
+      uint32_t nb = 0, slot = 0;  // key blocks before this one, ring slot of its first chunk
+      uint32_t nq = 0, turn = 0, np = 0, nfix = 0;  // phases
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (ok) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity));
+        tc::tc_fence_after();
+      };
+      auto there = [&](uint32_t g) { wait(&full[g % NG], (g / NG) & 1); };
+      auto q_there = [&](int qb) {
+        wait(&q_full[qb], (nq >> qb) & 1);
+        nq ^= 1u << qb;
+      };
+      auto p_there = [&](int x) {
+        wait(&p_full[x], (np >> x) & 1);
+        np ^= 1u << x;
+      };
+      auto fixed = [&]() { wait(v_fixed, nfix++ & 1); };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) tc::tc_commit(bar);
+      };
+      auto wrap = [](uint32_t sl) -> uint32_t { return sl >= (uint32_t)NS ? sl - NS : sl; };
+      // S = Q K^T of tile x from Q buffer qb and the K chunks at ring slot `at`
+      auto issue_s = [&](int x, int qb, uint32_t at) {
+        const uint32_t d = tb + x * 128;
+        if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < S::QCH; ++c) {
             const uint32_t a = aq + (qb * S::QB + c * S::QCHUNK) / 16, b = bk + wrap(at + c) * (kChunk / 16);
@@ -604,10 +656,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             for (int kk = 0; kk < 4; ++kk) mma_ss(d, a + kk * 2, b + kk * 2, idesc_s, (c | kk) != 0);
           }
           tc::tc_commit(&s_full[x]);
-        };
-        // O += P V of tile x from the V chunks at ring slot `at`
-        auto issue_pv = [&](int x, uint32_t at, bool first) {
-          const uint32_t d = tbase + 256 + x * DV, a = tbase + x * 128;
+        }
+        __syncwarp();
+      };
+      // O += P V of tile x from the V chunks at ring slot `at`
+      auto issue_pv = [&](int x, uint32_t at, bool first) {
+        const uint32_t d = tb + 256 + x * DV, a = tb + x * 128;
+        if (elect_one()) {
           if (S::VCH == 1 || at + 1 < (uint32_t)NS) {  // the V chunks lie one behind the other
             const uint32_t b = bv + at * (kChunk / 16);
 #pragma unroll
@@ -620,93 +675,96 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               for (int kk = 0; kk < 8; ++kk) mma_ts(d + c * 64, a + kk * 8, b + kk * 128, idesc_o64, kk != 0 || !first);
             }
           }
+        }
+        __syncwarp();
+      };
+      for (int s = 0; s < nseg && ok; ++s) {
+        Seg g = list.next();
+        g.ntok = __shfl_sync(0xFFFFFFFFu, g.ntok, 0), g.qfirst = __shfl_sync(0xFFFFFFFFu, g.qfirst, 0);
+        g.b0 = __shfl_sync(0xFFFFFFFFu, g.b0, 0), g.nblk = __shfl_sync(0xFFFFFFFFu, g.nblk, 0);
+        const int qlast = g.qfirst + g.ntok - 1;
+        const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
+        // block j of the unit has V rows that are nobody's
+        auto ragged = [&](int j) -> bool {
+          const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb), kp = kb * 128;
+          return !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
         };
-        for (int s = 0; s < nseg && ok; ++s) {
-          const Seg g = load_seg(s);
-          const int qlast = g.qfirst + g.ntok - 1;
-          const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
-          // block j of the unit has V rows that are nobody's
-          auto ragged = [&](int j) -> bool {
-            const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb), kp = kb * 128;
-            return !(kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep));
-          };
-          if (LIST == kLarge && g.ntok > tpt) {  // a pair: both tiles on every block
-            there(2 * nb);
+        auto request_fix = [&]() {
+          if (ok && elect_one()) mbar_arrive(fix_req);
+        };
+        if (LIST == kLarge && g.ntok > tpt) {  // a pair: both tiles on every block
+          there(2 * nb);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            q_there(x);
+            if (!ok) break;
+            issue_s(x, x, slot);
+            if (g.nblk == 1) commit(&q_empty[x]);
+          }
+          commit(&empty[(2 * nb) % NG]);
+          for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
+            const uint32_t vs = wrap(slot + S::QCH), next = wrap(vs + S::VCH);
+            const bool more = j + 1 < g.nblk, fix = ragged(g.b0 + j);
+            there(2 * nb + 1);
+            if (fix) request_fix();  // zeroed while the softmax runs
+            if (more) there(2 * nb + 2);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              q_there(x);
-              if (!ok) break;
-              issue_s(x, x, slot);
-              if (g.nblk == 1) tc::tc_commit(&q_empty[x]);
-            }
-            tc::tc_commit(&empty[(2 * nb) % NG]);
-            for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
-              const uint32_t vs = wrap(slot + S::QCH), next = wrap(vs + S::VCH);
-              const bool more = j + 1 < g.nblk, fix = ragged(g.b0 + j);
-              there(2 * nb + 1);
-              if (fix && ok) mbar_arrive(fix_req);  // zeroed while the softmax runs
-              if (more) there(2 * nb + 2);
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                p_there(x);
-                if (x == 0 && fix) fixed();
-                if (!ok) break;
-                tc::tc_fence_after();
-                issue_pv(x, vs, j == 0);
-                if (x == 1) tc::tc_commit(&empty[(2 * nb + 1) % NG]);
-                if (more) {
-                  issue_s(x, x, next);
-                  if (x == 1) tc::tc_commit(&empty[(2 * nb + 2) % NG]);
-                  if (j + 2 == g.nblk) tc::tc_commit(&q_empty[x]);
-                } else {
-                  tc::tc_commit(&o_full[x]);
-                }
-              }
-              slot = next;
-            }
-          } else {  // one tile: blocks in turn as A and B
-            const uint32_t qb = turn;
-            turn ^= 1;
-            const uint32_t nb0 = nb;
-            uint32_t ks = slot, kb = nb;  // the next block whose S is issued
-            auto issue_next = [&](int x) {
-              there(2 * kb);
-              if (!ok) return;
-              issue_s(x, qb, ks);
-              tc::tc_commit(&empty[(2 * kb) % NG]);
-              ks = wrap(ks + CPB);
-              if (++kb == nb0 + g.nblk) tc::tc_commit(&q_empty[qb]);
-            };
-            q_there(qb);
-            issue_next(0);
-            if (g.nblk > 1) issue_next(1);
-            for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
-              const int x = j & 1;
-              const uint32_t vs = wrap(slot + S::QCH);
-              const bool fix = ragged(g.b0 + j);
-              there(2 * nb + 1);
-              if (fix && ok) mbar_arrive(fix_req);
               p_there(x);
-              if (fix) fixed();
+              if (x == 0 && fix) fixed();
               if (!ok) break;
-              tc::tc_fence_after();
-              issue_pv(x, vs, j < 2);
-              tc::tc_commit(&empty[(2 * nb + 1) % NG]);
-              // this block's V may have to leave the ring before that K can come
-              if (j + 2 < g.nblk) issue_next(x);
-              slot = wrap(vs + S::VCH);
+              issue_pv(x, vs, j == 0);
+              if (x == 1) commit(&empty[(2 * nb + 1) % NG]);
+              if (more) {
+                issue_s(x, x, next);
+                if (x == 1) commit(&empty[(2 * nb + 2) % NG]);
+                if (j + 2 == g.nblk) commit(&q_empty[x]);
+              } else {
+                commit(&o_full[x]);
+              }
             }
-            tc::tc_commit(&o_full[0]);
-            tc::tc_commit(&o_full[1]);
+            slot = next;
           }
+        } else {  // one tile: blocks in turn as A and B
+          const uint32_t qb = turn, nb0 = nb;
+          turn ^= 1;
+          uint32_t ks = slot, kb = nb;  // the next block whose S is issued
+          auto issue_next = [&](int x) {
+            there(2 * kb);
+            if (!ok) return;
+            issue_s(x, qb, ks);
+            commit(&empty[(2 * kb) % NG]);
+            ks = wrap(ks + CPB);
+            if (++kb == nb0 + g.nblk) commit(&q_empty[qb]);
+          };
+          q_there(qb);
+          issue_next(0);
+          if (g.nblk > 1) issue_next(1);
+          for (int j = 0; j < g.nblk && ok; ++j, ++nb) {
+            const int x = j & 1;
+            const uint32_t vs = wrap(slot + S::QCH);
+            const bool fix = ragged(g.b0 + j);
+            there(2 * nb + 1);
+            if (fix) request_fix();
+            p_there(x);
+            if (fix) fixed();
+            if (!ok) break;
+            issue_pv(x, vs, j < 2);
+            commit(&empty[(2 * nb + 1) % NG]);
+            // this block's V may have to leave the ring before that K can come
+            if (j + 2 < g.nblk) issue_next(x);
+            slot = wrap(vs + S::VCH);
+          }
+          commit(&o_full[0]);
+          commit(&o_full[1]);
         }
-        tc::tc_commit(drain);  // every MMA issued above has completed once this arrives
-        if (!mbar_wait(drain, 0)) ok = false;
       }
+      commit(drain);  // every MMA issued above has completed once this arrives
+      if (!mbar_wait(drain, 0)) ok = false;
     } else if (warp == 10) {  // --------------------------------------------------- zeroes what nobody sees of V
       uint32_t ci = 0, fixes = 0;
       for (int s = 0; s < nseg && ok; ++s) {
-        const Seg g = load_seg(s);
+        const Seg g = list.next();
         const int qlast = g.qfirst + g.ntok - 1;
         const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
         for (int j = 0; j < g.nblk && ok; ++j, ci += CPB) {
@@ -716,16 +774,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           ok = mbar_wait(fix_req, fixes++ & 1);  // the block's V is there
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
+          // pages nobody sees hold zeros already; what is left are rows of the pages at the ends of what is seen
+          auto zero = [&](int from, int to) {
+            from = max(from, kp), to = min(to, kp + 128);
+            for (int i = from * 8 + lane; i < to * 8; i += 32) {  // a row is 128 bytes whatever the swizzle
 #pragma unroll
-          for (int c = 0; c < S::VCH; ++c) {
-            uint8_t* chunk = sRing + ((ci + S::QCH + c) % NS) * kChunk;
-            // a row is 128 bytes whatever the swizzle: 8 lanes a row
-            for (int row = lane >> 3; row < 128; row += 4) {
-              const int pos = kp + row;
-              if (pos > qlast || (pos < bl.lo && pos >= bl.keep))
-                *reinterpret_cast<uint4*>(chunk + row * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+              for (int c = 0; c < S::VCH; ++c)
+                *reinterpret_cast<uint4*>(sRing + ((ci + S::QCH + c) % NS) * kChunk + (i - kp * 8) * 16) =
+                    make_uint4(0, 0, 0, 0);
             }
-          }
+          };
+          const int in_page = (1 << p.page_shift) - 1;
+          zero(qlast + 1, (qlast | in_page) + 1);
+          zero(max(bl.lo & ~in_page, bl.keep), bl.lo);
+          if (bl.keep > 0) zero(bl.keep, min((bl.keep - 1 | in_page) + 1, bl.lo));
           tc::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(v_fixed);
@@ -741,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     const float sl2 = p.scale_log2;
     uint32_t ns = 0, no = 0;
     for (int s = 0; s < nseg; ++s) {
-      const Seg g = load_seg(s);
+      const Seg g = list.next();
       const bool pair = LIST == kLarge && g.ntok > tpt;
       const int tt = r / p.G + (pair ? x * tpt : 0);  // its token of the unit
       const Blocks bl = blocks_of(g.qfirst, g.qfirst + g.ntok - 1, p.window, p.keep);
@@ -751,7 +813,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int qpos = row_ok ? g.qfirst + tt : 0x7FFFFFFF;
       const int lo = p.window > 0 && row_ok ? max(0, qpos - p.window + 1) : 0;
       const int keep = min(p.keep, lo);
-      float m_ref = -INFINITY, l = 0.f;
+      float m_ref = -INFINITY, m_new = -INFINITY, l = 0.f;
+      const float sink = p.sinks && row_ok ? p.sinks[g.hk * p.G + head] * kLog2e : 0.f;
       // after a wait that ran out the loops go on without work, for the barriers that both groups must pass
       for (int j = pair ? 0 : x; j < g.nblk; j += pair ? 1 : 2) {
         if (ok) ok = mbar_wait(&s_full[x], ns & 1);
@@ -760,70 +823,92 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         if (!ok) continue;
         tc::tc_fence_after();
         if (work) {
-          float v[128];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, v + c * 32);
-          tc::tmem_wait_ld();
           const int jb = g.b0 + j, kp = (jb < bl.nkb ? jb : bl.lb + (jb - bl.nkb)) * 128;
-          if (!(kp + 127 <= qpos && (kp >= lo || kp + 127 < keep))) {
-            // 32 columns at a time as a word of visible bits: [c_lo, c_hi] and [0, c_keep)
-            const int c_hi = qpos - kp, c_lo = lo - kp, c_keep = keep - kp;
+          const bool masked = !(kp + 127 <= qpos && (kp >= lo || kp + 127 < keep));
+          // 32 columns at a time as a word of visible bits: [c_lo, c_hi] and [0, c_keep)
+          auto mask = [&](float* v, int w0) {
+            const int c_hi = qpos - kp - w0, c_lo = lo - kp - w0, c_keep = keep - kp - w0;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < 2; ++w) {
               auto below = [&](int c) -> uint32_t {  // bits of the columns < c
                 const int k = min(max(c - w * 32, 0), 32);
                 return k == 32 ? 0xFFFFFFFFu : (1u << k) - 1u;
               };
               const uint32_t seen = below(min(c_hi, 0x7FFFFFFE) + 1) & (~below(c_lo) | below(c_keep));
+              if (seen != 0xFFFFFFFFu) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(seen & (1u << e))) v[w * 32 + e] = -INFINITY;
+                for (int e = 0; e < 32; ++e)
+                  if (!(seen & (1u << e))) v[w * 32 + e] = -INFINITY;
+              }
             }
-          }
-          float mx[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float a = v[c * 32];
-#pragma unroll
-            for (int e = 1; e < 32; ++e) a = fmaxf(a, v[c * 32 + e]);
-            mx[c] = a;
-          }
-          // the scale is positive, so it orders the scaled scores alike
-          const float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sl2;
-          float alpha = 1.f;
-          bool rescale = false;
-          if (m > -INFINITY) {
-            if (m_ref == -INFINITY) {
-              m_ref = m;
-            } else if (m > m_ref + 8.f) {
-              alpha = ex2_approx(m_ref - m);
-              m_ref = m;
-              rescale = true;
-            }
-          }
-          const float nm = m_ref == -INFINITY ? 0.f : -m_ref;
-          float sum[4] = {0.f, 0.f, 0.f, 0.f};
-          uint32_t pk[64];
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            const float p0 = ex2_approx(fmaf(v[2 * i], sl2, nm)), p1 = ex2_approx(fmaf(v[2 * i + 1], sl2, nm));
-            sum[i & 3] += p0 + p1;
-            pk[i] = pack_bf16x2_rn(p0, p1);  // P is rounded to bf16 for the product with V, the sum is not
-          }
-          l = l * alpha + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
-          if (__any_sync(0xFFFFFFFFu, rescale)) {  // O holds the product of the block before (see above)
+          };
+          float v0[64], v1[64];  // scores of the block's halves
+          tmem_ld32(tS, v0);
+          tmem_ld32(tS + 32, v0 + 32);
+          tmem_ld32(tS + 64, v1);
+          tmem_ld32(tS + 96, v1 + 32);
+          tc::tmem_wait_ld();
+          if (masked) mask(v0, 0), mask(v1, 64);
+          // A new reference: O, which holds the products of the blocks before (see above), and the sum are scaled to it.
+          auto refer = [&](float to, bool mine) {
+            const float alpha = mine && m_ref != -INFINITY ? ex2_approx(m_ref - to) : 1.f;
+            if (mine) m_ref = to;
+            l *= alpha;
+            if (!__any_sync(0xFFFFFFFFu, alpha != 1.f)) return;
 #pragma unroll 1
-            for (int c = 0; c < DV; c += 32) {
-              float o[32];
-              tmem_ld32(tO + c, o);
+            for (int c = 0; c < DV; c += 16) {
+              float o[16];
+              tc::tmem_ld<16>(tO + c, o);
               tc::tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] *= alpha;
-              tmem_st32(tO + c, reinterpret_cast<const uint32_t*>(o));
+              for (int e = 0; e < 16; ++e) o[e] *= alpha;
+              tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
             }
+          };
+          // The reference of the exponentials is a maximum of the blocks before: a bf16 or float32 value is as exact
+          // beside 2^60 as beside 1, so the exponentials need not wait for this block's maximum.  A maximum 2^8 above
+          // it is taken up at the next block, one 2^60 above it (and the first block's) at once.
+          if (__any_sync(0xFFFFFFFFu, m_new > m_ref + 8.f)) refer(m_new, m_new > m_ref + 8.f);
+          uint32_t pk[32];
+          uint64_t sum[2];
+          auto half = [&](const float* v) {  // 64 columns: P = bf16(2^(s * scale * log2 e - reference)), and their sum
+            const uint64_t sc = pack2(sl2, sl2), nm = m_ref == -INFINITY ? 0 : pack2(-m_ref, -m_ref);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float2 t = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), sc, nm));
+              const float p0 = ex2_approx(t.x), p1 = ex2_approx(t.y);
+              sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
+              pk[i] = pack_bf16x2_rn(p0, p1);  // rounded to bf16 for the product with V, the sum is not
+            }
+          };
+          auto maximum = [&](const float* v) -> float {
+            float a = v[0], b = v[1];
+#pragma unroll
+            for (int e = 2; e < 62; e += 4) a = fmaxf(fmaxf(a, v[e]), v[e + 1]), b = fmaxf(fmaxf(b, v[e + 2]), v[e + 3]);
+            return fmaxf(fmaxf(a, v[62]), fmaxf(b, v[63]));
+          };
+          // the scale is positive, so it orders the scaled scores alike
+          if (__any_sync(0xFFFFFFFFu, m_ref == -INFINITY)) {
+            const float m = fmaxf(maximum(v0), maximum(v1)) * sl2;
+            refer(m, m_ref == -INFINITY && m > -INFINITY);
+          }
+          sum[0] = sum[1] = 0;
+          m_new = fmaxf(maximum(v0), maximum(v1)) * sl2;
+          half(v0);
+          if (__any_sync(0xFFFFFFFFu, m_new > m_ref + 60.f)) {
+            refer(m_new, m_new > m_ref + 8.f);
+            tmem_ld32(tS, v0);
+            tmem_ld32(tS + 32, v0 + 32);
+            tc::tmem_wait_ld();
+            if (masked) mask(v0, 0);
+            sum[0] = sum[1] = 0;
+            half(v0);
           }
           tmem_st32(tS, pk);
-          tmem_st32(tS + 32, pk + 32);
+          half(v1);
+          const float2 s0 = unpack2(add2(sum[0], sum[1]));
+          l += s0.x + s0.y;
+          tmem_st32(tS + 32, pk);
           tmem_wait_st();
         }
         tc::tc_fence_before();
@@ -855,10 +940,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         float f = 1.f;  // an unnormalised part: maximum (log2), sum and output of these blocks
         if (g.slot < 0) {
           if (p.sinks) {
-            const float sk = (row_ok ? p.sinks[qh] : 0.f) * kLog2e;
-            const float M = fmaxf(m_ref, sk);
+            const float M = fmaxf(m_ref, sink);
             const float a = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
-            f = a / (l * a + exp2f(sk - M));
+            f = a / (l * a + exp2f(sink - M));
           } else {
             f = l == 0.f ? 0.f : 1.f / l;
           }
@@ -868,15 +952,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
 #pragma unroll 1
         for (int c = c0; c < c1; c += 32) {
-          float o[32];
+          float o[32], q[32];
           tmem_ld32(tO + c, o);
+          if (!pair) tmem_ld32(tOther + c, q);
           tc::tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = own ? o[e] * w_own : 0.f;
           if (!pair) {
-            float q[32];
-            tmem_ld32(tOther + c, q);
-            tc::tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
           }
