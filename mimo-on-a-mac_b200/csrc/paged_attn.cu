@@ -707,7 +707,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             const bool more = j + 1 < g.nblk, fix = ragged(g.b0 + j);
             there(2 * nb + 1);
             if (fix) request_fix();  // zeroed while the softmax runs
-            if (more) there(2 * nb + 2);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               p_there(x);
@@ -716,6 +715,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               issue_pv(x, vs, j == 0);
               if (x == 1) commit(&empty[(2 * nb + 1) % NG]);
               if (more) {
+                if (x == 0) there(2 * nb + 2);
+                if (!ok) break;
                 issue_s(x, x, next);
                 if (x == 1) commit(&empty[(2 * nb + 2) % NG]);
                 if (j + 2 == g.nblk) commit(&q_empty[x]);
@@ -814,6 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int lo = p.window > 0 && row_ok ? max(0, qpos - p.window + 1) : 0;
       const int keep = min(p.keep, lo);
       float m_ref = -INFINITY, m_new = -INFINITY, l = 0.f;
+      bool fresh = true;
       const float sink = p.sinks && row_ok ? p.sinks[g.hk * p.G + head] * kLog2e : 0.f;
       // after a wait that ran out the loops go on without work, for the barriers that both groups must pass
       for (int j = pair ? 0 : x; j < g.nblk; j += pair ? 1 : 2) {
@@ -868,44 +870,48 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           // The reference of the exponentials is a maximum of the blocks before: a bf16 or float32 value is as exact
           // beside 2^60 as beside 1, so the exponentials need not wait for this block's maximum.  A maximum 2^8 above
           // it is taken up at the next block, one 2^60 above it (and the first block's) at once.
-          if (__any_sync(0xFFFFFFFFu, m_new > m_ref + 8.f)) refer(m_new, m_new > m_ref + 8.f);
+          // (rows without a query have no say: what they compute on may be anything)
+          const bool later = row_ok && m_new > m_ref + 8.f;
+          if (__any_sync(0xFFFFFFFFu, later)) refer(m_new, later);
           uint32_t pk[32];
           uint64_t sum[2];
-          auto half = [&](const float* v) {  // 64 columns: P = bf16(2^(s * scale * log2 e - reference)), and their sum
+          // 64 columns: P = bf16(2^(s * scale * log2 e - reference)) and their sum; with `mx`, the maximum of both halves
+          // on the way (the scale is positive, so it orders the scaled scores alike).  The special-function unit bounds
+          // this loop, and what else it does has to lie between its instructions.
+          auto half = [&](const float* v, const float* u, float* mx) {
             const uint64_t sc = pack2(sl2, sl2), nm = m_ref == -INFINITY ? 0 : pack2(-m_ref, -m_ref);
+            float a = -INFINITY, b = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float2 t = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), sc, nm));
               const float p0 = ex2_approx(t.x), p1 = ex2_approx(t.y);
+              if (mx) a = fmaxf(fmaxf(a, v[2 * i]), v[2 * i + 1]), b = fmaxf(fmaxf(b, u[2 * i]), u[2 * i + 1]);
               sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
               pk[i] = pack_bf16x2_rn(p0, p1);  // rounded to bf16 for the product with V, the sum is not
             }
+            if (mx) *mx = fmaxf(a, b) * sl2;
           };
-          auto maximum = [&](const float* v) -> float {
-            float a = v[0], b = v[1];
+          if (fresh) {  // rows without a reference yet: the unit's first block, and rows that have seen no key so far
+            float a = -INFINITY;
 #pragma unroll
-            for (int e = 2; e < 62; e += 4) a = fmaxf(fmaxf(a, v[e]), v[e + 1]), b = fmaxf(fmaxf(b, v[e + 2]), v[e + 3]);
-            return fmaxf(fmaxf(a, v[62]), fmaxf(b, v[63]));
-          };
-          // the scale is positive, so it orders the scaled scores alike
-          if (__any_sync(0xFFFFFFFFu, m_ref == -INFINITY)) {
-            const float m = fmaxf(maximum(v0), maximum(v1)) * sl2;
-            refer(m, m_ref == -INFINITY && m > -INFINITY);
+            for (int e = 0; e < 64; ++e) a = fmaxf(fmaxf(a, v0[e]), v1[e]);
+            a *= sl2;
+            refer(a, row_ok && m_ref == -INFINITY && a > -INFINITY);
+            fresh = __any_sync(0xFFFFFFFFu, row_ok && m_ref == -INFINITY);
           }
           sum[0] = sum[1] = 0;
-          m_new = fmaxf(maximum(v0), maximum(v1)) * sl2;
-          half(v0);
-          if (__any_sync(0xFFFFFFFFu, m_new > m_ref + 60.f)) {
-            refer(m_new, m_new > m_ref + 8.f);
+          half(v0, v1, &m_new);
+          if (__any_sync(0xFFFFFFFFu, row_ok && m_new > m_ref + 60.f)) {
+            refer(m_new, row_ok && m_new > m_ref + 8.f);
             tmem_ld32(tS, v0);
             tmem_ld32(tS + 32, v0 + 32);
             tc::tmem_wait_ld();
             if (masked) mask(v0, 0);
             sum[0] = sum[1] = 0;
-            half(v0);
+            half(v0, v1, nullptr);
           }
           tmem_st32(tS, pk);
-          half(v1);
+          half(v1, v0, nullptr);
           const float2 s0 = unpack2(add2(sum[0], sum[1]));
           l += s0.x + s0.y;
           tmem_st32(tS + 32, pk);
