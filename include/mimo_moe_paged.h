@@ -75,7 +75,8 @@ int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_hea
  * lengths do not fit (more rows than positions, more positions than its table row, rows outside `tokens`) sets
  * MIMO_ERANGE and gets no output.  The attention must be given the arguments that its plan was made with (otherwise
  * status becomes MIMO_ERANGE and nothing is computed) on the same GPU; a page outside the pool sets MIMO_ERANGE and
- * reads as zeros.  workspace: ..._workspace_bytes, 16-byte aligned, for one call at a time. */
+ * reads as zeros.  workspace: ..._workspace_bytes, for one call at a time; out and workspace are
+ * 32-byte aligned. */
 size_t mimo_moe_paged_attention_plan_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads);
 int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, int32_t R, int32_t tokens,
                                   int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,

@@ -1036,6 +1036,7 @@ int mimo_moe_profile_read(int32_t* launches, float* milliseconds) {
 // ------------------------------------------------------------- decoder layer (include/mimo_moe_layer.h)
 namespace {
 bool a16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+bool a32(const void* p) { return ((uintptr_t)p & 31) == 0; }
 size_t attn_split_bytes(int32_t T, int32_t nq, int32_t dv) { return (size_t)T * nq * ((size_t)dv + 2) * 4; }
 }  // namespace
 
@@ -1257,7 +1258,7 @@ int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const u
       bad_heads(n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
       keep_first < 0 || (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) ||
       (int64_t)num_pages * n_kv_heads >= INT32_MAX || bad_table(R, table_width, page_size) || !a16(q) ||
-      !a16(k_pages) || !a16(v_pages) || !a16(out) || !a16(plan) || !a16(workspace) ||
+      !a16(k_pages) || !a16(v_pages) || !a32(out) || !a16(plan) || !a32(workspace) ||
       plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads) ||
       workspace_bytes < mimo_moe_paged_attention_workspace_bytes(tokens, R, n_heads, n_kv_heads, v_head_dim))
     return MIMO_EINVAL;

@@ -26,6 +26,7 @@
 //                    hold anything, and 0 * NaN is not 0.
 // Every wait is bounded and sets MIMO_ETIMEOUT; the producer drains its copies and the issuer its MMAs before exit.
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -414,6 +415,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
+// 32 bytes, 32-byte aligned: a whole sector.
+__device__ __forceinline__ void st_global_v8(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // True in one lane of the warp, which must be whole here.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -956,32 +963,75 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         w_own *= f, w_other *= f;
         const bool store = row_ok && row < p.T;
         const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 32) {
-          float o[32], q[32];
-          tmem_ld32(tO + c, o);
-          if (!pair) tmem_ld32(tOther + c, q);
-          tc::tmem_wait_ld();
+        // N columns from c on: scaled, joined, written
+        auto emit = [&](auto n, int c) {
+          constexpr int N = decltype(n)::value;
+          float o[N];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = own ? o[e] * w_own : 0.f;
-          if (!pair) {
+          for (int k = 0; k < N; k += 32) tmem_ld32(tO + c + k, o + k);
+          if (pair) {
+            tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
+            for (int e = 0; e < N; ++e) o[e] *= w_own;
+          } else {
+            float q[N];
+#pragma unroll
+            for (int k = 0; k < N; k += 32) tmem_ld32(tOther + c + k, q + k);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+              o[e] = own ? o[e] * w_own : 0.f;
+              o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
+            }
           }
-          if (store && g.slot < 0) {
-            uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)row * p.nq + qh) * DV + c);
+          if (g.slot >= 0) {
+            if (store)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4];
+              for (int e = 0; e < N; e += 8) st_global_v8(p.part_o + at * DV + c + e, reinterpret_cast<uint32_t*>(o + e));
+            return;
+          }
+          uint32_t w[N / 2];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) w[k] = pack_bf16x2_rn(o[e * 8 + 2 * k], o[e * 8 + 2 * k + 1]);
-              dst[e] = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < N / 2; ++e) w[e] = pack_bf16x2_rn(o[2 * e], o[2 * e + 1]);
+          uint16_t* dst = p.out + ((size_t)row * p.nq + qh) * DV + c;
+          if constexpr (N == 64) {
+            // A row is 128 bytes here.  A store of one piece of 32 different rows takes the load/store unit 32 turns (a
+            // unit's 128 x 128 outputs took 7600 cycles that way), so the four lanes of a quad first exchange theirs:
+            // chunk q (32 bytes) of the quad's rows goes to lane q, and a store writes whole rows.
+            const int q = lane & 3;
+#pragma unroll
+            for (int st = 0; st < 2; ++st) {
+              const bool hi = (q >> st) & 1;
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if ((k >> st) & 1) continue;
+                const int k1 = k | (1 << st);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  const uint32_t give = hi ? w[k * 8 + e] : w[k1 * 8 + e];
+                  const uint32_t take = __shfl_xor_sync(0xFFFFFFFFu, give, 1 << st);
+                  w[k * 8 + e] = hi ? take : w[k * 8 + e];
+                  w[k1 * 8 + e] = hi ? w[k1 * 8 + e] : take;
+                }
+              }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const bool yes = __shfl_sync(0xFFFFFFFFu, (int)store, (lane & ~3) | k) != 0;
+              uint16_t* to = reinterpret_cast<uint16_t*>(
+                  __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), (lane & ~3) | k));
+              if (yes) st_global_v8(to + q * 16, w + k * 8);
             }
           } else if (store) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + at * DV + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < N / 2; e += 8) st_global_v8(dst + e * 2, w + e);
           }
+        };
+        if (DV == 64 && !pair) {
+          emit(std::integral_constant<int, 32>{}, c0);
+        } else {
+#pragma unroll 1
+          for (int c = c0; c < c1; c += 64) emit(std::integral_constant<int, 64>{}, c);
         }
         if (store && g.slot >= 0 && c0 == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
       }

@@ -79,7 +79,7 @@ def test_paged_attention_plan_refuses(bad):
                                  dict(nq=258, nkv=2), dict(d=96), dict(dv=192), dict(d=64), dict(scale=0.0),
                                  dict(scale=float("nan")), dict(window=-1), dict(keep=-1), dict(window=0, keep=4),
                                  dict(pages=0), dict(P=24), dict(width=0), dict(q=A + 8), dict(k=A + 2), dict(v=A + 8),
-                                 dict(out=A + 8), dict(plan=A + 4), dict(ws=A + 4), dict(nb=-1), dict(wb=-1),
+                                 dict(out=A + 16), dict(plan=A + 4), dict(ws=A + 16), dict(nb=-1), dict(wb=-1),
                                  dict(pages=1 << 26, nq=256, nkv=128, T=1)])
 def test_paged_attention_refuses(bad):
     L = _lib()
