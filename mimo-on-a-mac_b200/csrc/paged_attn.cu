@@ -415,6 +415,9 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};\n" ::"r"(taddr), "r"(r) : "memory");
+}
 // 32 bytes, 32-byte aligned: a whole sector.
 __device__ __forceinline__ void st_global_v8(void* p, const uint32_t* r) {
   asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
@@ -851,13 +854,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               }
             }
           };
-          float v0[64], v1[64];  // scores of the block's halves
-          tmem_ld32(tS, v0);
-          tmem_ld32(tS + 32, v0 + 32);
-          tmem_ld32(tS + 64, v1);
-          tmem_ld32(tS + 96, v1 + 32);
-          tc::tmem_wait_ld();
-          if (masked) mask(v0, 0), mask(v1, 64);
           // A new reference: O, which holds the products of the blocks before (see above), and the sum are scaled to it.
           auto refer = [&](float to, bool mine) {
             const float alpha = mine && m_ref != -INFINITY ? ex2_approx(m_ref - to) : 1.f;
@@ -873,55 +869,77 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               for (int e = 0; e < 16; ++e) o[e] *= alpha;
               tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
             }
+            tmem_wait_st();
           };
-          // The reference of the exponentials is a maximum of the blocks before: a bf16 or float32 value is as exact
-          // beside 2^60 as beside 1, so the exponentials need not wait for this block's maximum.  A maximum 2^8 above
-          // it is taken up at the next block, one 2^60 above it (and the first block's) at once.
+          // The reference of the exponentials is a maximum of what came before: a bf16 or float32 value is as exact beside
+          // 2^60 as beside 1, so the exponentials need not wait for their own maximum.  A maximum 2^8 above the reference
+          // is taken up at the next block, one 2^60 above it (and a row's first) at once.
           // (rows without a query have no say: what they compute on may be anything)
           const bool later = row_ok && m_new > m_ref + 8.f;
           if (__any_sync(0xFFFFFFFFu, later)) refer(m_new, later);
-          uint32_t pk[32];
-          uint64_t sum[2];
-          // 64 columns: P = bf16(2^(s * scale * log2 e - reference)) and their sum; with `mx`, the maximum of both halves
-          // on the way (the scale is positive, so it orders the scaled scores alike).  The special-function unit bounds
-          // this loop, and what else it does has to lie between its instructions.
-          auto half = [&](const float* v, const float* u, float* mx) {
-            const uint64_t sc = pack2(sl2, sl2), nm = m_ref == -INFINITY ? 0 : pack2(-m_ref, -m_ref);
-            float a = -INFINITY, b = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float2 t = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), sc, nm));
-              const float p0 = ex2_approx(t.x), p1 = ex2_approx(t.y);
-              if (mx) a = fmaxf(fmaxf(a, v[2 * i]), v[2 * i + 1]), b = fmaxf(fmaxf(b, u[2 * i]), u[2 * i + 1]);
-              sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
-              pk[i] = pack_bf16x2_rn(p0, p1);  // rounded to bf16 for the product with V, the sum is not
-            }
-            if (mx) *mx = fmaxf(a, b) * sl2;
-          };
-          if (fresh) {  // rows without a reference yet: the unit's first block, and rows that have seen no key so far
-            float a = -INFINITY;
-#pragma unroll
-            for (int e = 0; e < 64; ++e) a = fmaxf(fmaxf(a, v0[e]), v1[e]);
-            a *= sl2;
-            refer(a, row_ok && m_ref == -INFINITY && a > -INFINITY);
-            fresh = __any_sync(0xFFFFFFFFu, row_ok && m_ref == -INFINITY);
-          }
-          sum[0] = sum[1] = 0;
-          half(v0, v1, &m_new);
-          if (__any_sync(0xFFFFFFFFu, row_ok && m_new > m_ref + 60.f)) {
-            refer(m_new, row_ok && m_new > m_ref + 8.f);
-            tmem_ld32(tS, v0);
-            tmem_ld32(tS + 32, v0 + 32);
+          m_new = -INFINITY;
+          // The halves one after the other through the same instructions: written out for both, with the rare repetition,
+          // the loop was larger than the instruction caches hold, and the warps waited for it.
+#pragma unroll 1
+          for (int hf = 0; hf < 2; ++hf) {
+            float v[64];
+            tmem_ld32(tS + hf * 64, v);
+            tmem_ld32(tS + hf * 64 + 32, v + 32);
             tc::tmem_wait_ld();
-            if (masked) mask(v0, 0);
-            sum[0] = sum[1] = 0;
-            half(v0, v1, nullptr);
+            if (masked) mask(v, hf * 64);
+            if (fresh) {  // rows without a reference yet: the unit's first block, and rows that have seen no key so far
+              float a = v[0];
+#pragma unroll
+              for (int e = 1; e < 63; e += 2) a = fmaxf(fmaxf(a, v[e]), v[e + 1]);
+              a = fmaxf(a, v[63]) * sl2;
+              refer(a, row_ok && m_ref == -INFINITY && a > -INFINITY);
+              fresh = __any_sync(0xFFFFFFFFu, row_ok && m_ref == -INFINITY);
+            }
+            uint32_t pk[32];
+            uint64_t sum[2];
+            for (;;) {
+              // P = bf16(2^(s * scale * log2 e - reference)) and their sum, and their maximum on the way (the scale is
+              // positive, so it orders the scaled scores alike).  The special-function unit bounds this loop, and what
+              // else it does has to lie between its instructions.
+              const uint64_t sc = pack2(sl2, sl2), nm = m_ref == -INFINITY ? 0 : pack2(-m_ref, -m_ref);
+              float a = -INFINITY, b = -INFINITY;
+              sum[0] = sum[1] = 0;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                const float2 t = unpack2(fma2(pack2(v[2 * i], v[2 * i + 1]), sc, nm));
+                const float p0 = ex2_approx(t.x), p1 = ex2_approx(t.y);
+                if (i & 1) b = fmaxf(fmaxf(b, v[2 * i]), v[2 * i + 1]);
+                else a = fmaxf(fmaxf(a, v[2 * i]), v[2 * i + 1]);
+                sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
+                pk[i] = pack_bf16x2_rn(p0, p1);  // rounded to bf16 for the product with V, the sum is not
+              }
+              const float m = fmaxf(a, b) * sl2;
+              const bool jump = row_ok && m > m_ref + 60.f;
+              m_new = fmaxf(m_new, m);
+              if (!__any_sync(0xFFFFFFFFu, jump)) break;
+              const float was = m_ref;
+              refer(m, jump);
+              if (hf == 1) {  // the first half's P as well
+                const float alpha = jump && was != -INFINITY ? ex2_approx(was - m) : 1.f;
+                tmem_wait_st();
+#pragma unroll 1
+                for (int c = 0; c < 32; c += 8) {
+                  float w[8];
+                  tc::tmem_ld<8>(tS + c, w);
+                  tc::tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) {
+                    const uint32_t u = __float_as_uint(w[e]);
+                    const uint32_t z = pack_bf16x2_rn(__uint_as_float(u << 16) * alpha, __uint_as_float(u & 0xFFFF0000u) * alpha);
+                    tmem_st1(tS + c + e, z);
+                  }
+                }
+              }
+            }
+            const float2 s0 = unpack2(add2(sum[0], sum[1]));
+            l += s0.x + s0.y;
+            tmem_st32(tS + hf * 32, pk);
           }
-          tmem_st32(tS, pk);
-          half(v1, v0, nullptr);
-          const float2 s0 = unpack2(add2(sum[0], sum[1]));
-          l += s0.x + s0.y;
-          tmem_st32(tS + 32, pk);
           tmem_wait_st();
         }
         tc::tc_fence_before();
