@@ -18,6 +18,7 @@ and 8 on the 128-token sliding-window layers, sinks on the sliding-window layers
 from __future__ import annotations
 
 from dataclasses import dataclass, replace
+from functools import lru_cache
 from typing import Optional, Union
 
 import torch
@@ -57,6 +58,7 @@ def mimo_sliding_attention(**kw) -> AttentionConfig:
     return replace(AttentionConfig(n_kv_heads=8, rope_theta=10_000.0, window=128, sinks=True), **kw)
 
 
+@lru_cache(maxsize=None)
 def bf16_value(v: float) -> float:
     """The float a Python scalar becomes when MLX multiplies it into a bf16 array (cast to bf16)."""
     return float(torch.tensor(v, dtype=torch.float32).to(torch.bfloat16).to(torch.float32))

@@ -28,39 +28,40 @@ PAGE_SIZES = (16, 32, 64, 128)
 MAX_REQUESTS = 4096
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev: torch.device):
     """The context in which kernels launch on `dev` (nothing to do when it is the current device)."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)   # current_stream(dev).cuda_stream without the object
 
 
 def _int32(t: torch.Tensor, name: str, shape, dev=None) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.is_cuda and t.shape == shape and t.is_contiguous() and (dev is None
+                                                                                          or t.device == dev):
+        return t
     _need_cuda(t, name)
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, got {t.dtype} "
-                         f"{tuple(t.shape)}")
     if dev is not None and t.device != dev:
         raise ValueError(f"{name} is on {t.device}, the other tensors on {dev}")
-    return t
+    raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
 def _bf16(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
     """An activation input: any float type and layout, cast and made contiguous (no-ops for the layers' own)."""
-    _need_cuda(t, name)
-    if tuple(t.shape) != tuple(shape) or t.device != dev:
+    if t.shape != shape or t.device != dev:
+        _need_cuda(t, name)
         raise ValueError(f"{name} must have shape {tuple(shape)} on {dev}, got {tuple(t.shape)} on {t.device}")
-    return t.to(torch.bfloat16).contiguous()
+    return t if t.dtype is torch.bfloat16 and t.is_contiguous() else t.to(torch.bfloat16).contiguous()
 
 
 def _buffer(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
     """A tensor the kernels write: taken as it is."""
-    _need_cuda(t, name)
-    if tuple(t.shape) != tuple(shape) or t.device != dev or t.dtype != torch.bfloat16 or not t.is_contiguous():
+    if t.shape != shape or t.device != dev or t.dtype is not torch.bfloat16 or not t.is_cuda or not t.is_contiguous():
+        _need_cuda(t, name)
         raise ValueError(f"{name} must be a contiguous bf16 tensor of shape {tuple(shape)} on {dev}, got {t.dtype} "
                          f"{tuple(t.shape)} on {t.device}")
     return t
@@ -137,27 +138,24 @@ def page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Ten
     the end of free_pages[:n_free], writes them into block_table (in place) and returns the step's row layout.  lens
     and n_free stay as they are; the step's seq_lens and n_free are the new ones.  When the pages do not suffice, or a
     length does not fit, the step is one without new tokens and its status says so (PageStep.check)."""
-    dev, R = lens.device, block_table.shape[0]
-    page_size = _page_size(page_size)
-    _need_cuda(block_table, "block_table")
-    _int32(block_table, "block_table", block_table.shape)
     if out is None:
-        out = PageStep.empty(R, tokens, block_table, page_size)
-    elif (out.requests, out.tokens, out.page_size) != (R, tokens, page_size) or out.n_free is None \
-            or out.block_table.data_ptr() != block_table.data_ptr():
-        raise ValueError("page_plan: out is a step of other requests, rows, pages or another block table")
+        out = PageStep.empty(block_table.shape[0], tokens, block_table, page_size)
+    elif out.block_table is not block_table or out.tokens != tokens or out.page_size != page_size \
+            or out.n_free is None:
+        raise ValueError("page_plan: out is a step of other rows, pages or another block table")
+    R, dev = out.requests, out.device
     if free_pages.dim() != 1:
         raise ValueError("free_pages must be a vector")
-    _int32(lens, "lens", (R,), out.device)
-    _int32(new_lens, "new_lens", (R,), out.device)
-    _int32(free_pages, "free_pages", free_pages.shape, out.device)
-    _int32(n_free, "n_free", (1,), out.device)
+    _int32(lens, "lens", (R,), dev)
+    _int32(new_lens, "new_lens", (R,), dev)
+    _int32(free_pages, "free_pages", free_pages.shape, dev)
+    _int32(n_free, "n_free", (1,), dev)
     with _on(dev):
         check(lib().mimo_moe_page_plan(lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
-                                       block_table.shape[1], free_pages.data_ptr(), n_free.data_ptr(),
-                                       free_pages.shape[0], page_size, tokens, out.cu_q.data_ptr(),
-                                       out.seq_lens.data_ptr(), out.n_free.data_ptr(), out.positions.data_ptr(),
-                                       out.slots.data_ptr(), out.status.data_ptr(), _stream(dev)), "page_plan")
+                                       out.width, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0],
+                                       out.page_size, tokens, out.cu_q.data_ptr(), out.seq_lens.data_ptr(),
+                                       out.n_free.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(),
+                                       out.status.data_ptr(), _stream(dev)), "page_plan")
     return out
 
 
@@ -262,7 +260,9 @@ def _fits(cache: PagedKVCache, cfg: AttentionConfig, step: PageStep, where: str)
     if (cache.page_size, cache.device) != (step.page_size, step.device):
         raise ValueError(f"{where}: the cache has pages of {cache.page_size} on {cache.device}, the step pages of "
                          f"{step.page_size} on {step.device}")
-    if tuple(cache.k.shape[1::2]) != (cfg.n_kv_heads, cfg.head_dim) or cache.v.shape[3] != cfg.v_head_dim:
+    own = cache.cfg
+    if own is not cfg and (own.n_kv_heads, own.head_dim, own.v_head_dim) != (cfg.n_kv_heads, cfg.head_dim,
+                                                                             cfg.v_head_dim):
         raise ValueError(f"{where}: the cache was made for another attention config")
 
 
@@ -302,7 +302,7 @@ class AttentionPlan:
         if cfg.n_heads < 1 or cfg.n_kv_heads < 1 or cfg.n_heads % cfg.n_kv_heads or cfg.n_heads // cfg.n_kv_heads > 128:
             raise ValueError(f"attention_plan: {cfg.n_heads} heads over {cfg.n_kv_heads} kv heads")
         self.step, self.kind = step, _kind(cfg)
-        self.buffer = None
+        self.buffer, self._ws = None, {}
         if step.tokens == 0:
             return
         with _on(step.device):
@@ -310,6 +310,13 @@ class AttentionPlan:
             nb = L.mimo_moe_paged_attention_plan_bytes(step.tokens, step.requests, cfg.n_heads, cfg.n_kv_heads)
             self.buffer = torch.empty(nb, dtype=torch.uint8, device=step.device)
             self.update()
+
+    def workspace_bytes(self, v_head_dim: int) -> int:
+        nb = self._ws.get(v_head_dim)
+        if nb is None:
+            nb = self._ws[v_head_dim] = lib().mimo_moe_paged_attention_workspace_bytes(
+                self.step.tokens, self.step.requests, self.kind[0], self.kind[1], v_head_dim)
+        return nb
 
     def update(self) -> None:
         """Make the plan again from the step's present lengths, in the same buffer."""
@@ -351,16 +358,14 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
     if T == 0:
         return o
     with _on(dev):
-        L = lib()
-        nb = L.mimo_moe_paged_attention_workspace_bytes(T, step.requests, cfg.n_heads, cfg.n_kv_heads,
-                                                         cfg.v_head_dim)
+        nb = plan.workspace_bytes(cfg.v_head_dim)
         ws = torch.empty(nb, dtype=torch.uint8, device=dev)   # the call's own: two streams or graphs never share it
-        check(L.mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
-                                         step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,
-                                         cfg.n_kv_heads, cfg.head_dim, cfg.v_head_dim, float(cfg.scale), cfg.window,
-                                         cfg.keep_first, cache.num_pages, cache.page_size, plan.buffer.data_ptr(),
-                                         plan.buffer.numel(), o.data_ptr(), ws.data_ptr(), nb,
-                                         step.status.data_ptr(), _stream(dev)), "attention_paged")
+        check(lib().mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
+                                             step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,
+                                             cfg.n_kv_heads, cfg.head_dim, cfg.v_head_dim, float(cfg.scale),
+                                             cfg.window, cfg.keep_first, cache.num_pages, cache.page_size,
+                                             plan.buffer.data_ptr(), plan.buffer.numel(), o.data_ptr(), ws.data_ptr(),
+                                             nb, step.status.data_ptr(), _stream(dev)), "attention_paged")
     return o
 
 
