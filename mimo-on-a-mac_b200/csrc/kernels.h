@@ -353,6 +353,10 @@ struct AttnPlanParams {
   int merge_cost[2];                                     // of a split, in key blocks, for each list of units
   int key;                                               // what the plan was made for
 };
+struct PagedAttnList {  // where a list of work units lies: in the plan (words), and its parts in the workspace (rows)
+  size_t start, head, merge, segs, part0;
+  int part_rows;  // 0: the list has no units
+};
 struct PagedAttnParams {
   CUtensorMap qmap, kmap, vmap;  // q (box 64 dims x G heads x 128 / G tokens), pools (box 64 dims x a page)
   const uint16_t *q, *k, *v;     // q [T][nq][dqk], pools [num_pages][nkv][page][d]
@@ -363,6 +367,7 @@ struct PagedAttnParams {
   int32_t* status;
   int T, R, width, nq, nkv, G, dqk, dv, window, keep, num_pages, page_shift, key;
   int second;                    // the call's second attention kernel
+  PagedAttnList list[2];         // small units, others
   float scale_log2;              // softmax scale * log2(e)
 };
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms);

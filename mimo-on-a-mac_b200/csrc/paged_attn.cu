@@ -518,18 +518,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   if (!p.second) pdl_wait();
   pdl_launch_dependents();
 
-  const PlanLayout L = plan_layout(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
-  const int32_t* plan = p.plan + list_start(LIST, p.T, p.R, p.G, p.nkv, gridDim.x);
+  const int32_t* plan = p.plan + p.list[LIST].start;
   const int key = plan[0];
-  const int4* head = reinterpret_cast<const int4*>(plan + L.head) + 3 * blockIdx.x;
+  const int4* head = reinterpret_cast<const int4*>(plan + p.list[LIST].head) + 3 * blockIdx.x;
   const int4 where = head[0], first_a = head[1], first_b = head[2];
   const bool planned = key == p.key;  // a plan of these lengths' shape, this layer kind and this GPU
   if (!planned && threadIdx.x == 0) set_status(p.status, MIMO_ERANGE);
   const int nseg = planned ? where.y : 0;
-  const int4* segs = reinterpret_cast<const int4*>(plan + L.segs) + 2 * (size_t)where.x;
+  const int4* segs = reinterpret_cast<const int4*>(plan + p.list[LIST].segs) + 2 * (size_t)where.x;
   const int tpt = (LIST == kSmall ? kSmallRows : 128) / p.G;  // tokens per tile
-  const int part_rows = part_rows_of(LIST, p.T, p.R, p.G);
-  const size_t part0 = part_start(LIST, p.T, p.R, p.G, gridDim.x);
+  const int part_rows = p.list[LIST].part_rows;
+  const size_t part0 = p.list[LIST].part0;
   // the CTA's segments in turn, the next one's load in flight while one is worked on
   struct Segs {
     const int4* at;
@@ -1074,49 +1073,57 @@ constexpr int kMergeWarps = 8;
 
 template <int DV>
 __global__ void __launch_bounds__(kMergeWarps * 32) paged_attn_merge_kernel(const __grid_constant__ PagedAttnParams p) {
-  constexpr int VL = DV / 32;
+  constexpr int VL = DV / 32, AHEAD = 8;  // parts loaded at a time
+  // the plan is older than the attention kernels, which are all past their wait for it when this grid starts
+  const int list = p.list[kSmall].part_rows > 0 ? (int)blockIdx.z : kLarge;
+  const int32_t* plan = p.plan + p.list[list].start;
+  const int key = plan[0];
+  const int4* mg = reinterpret_cast<const int4*>(plan + p.list[list].merge) + 2 * (size_t)blockIdx.x;
+  const int4 a = mg[0], b = mg[1];  // row0, tokens, kv head, first CTA; slot of the first part, parts
+  const int part_rows = p.list[list].part_rows, lane = threadIdx.x & 31;
+  const size_t part0 = p.list[list].part0;
   pdl_wait();
   pdl_launch_dependents();
-  const int list = lists_of(p.T, p.R, p.G).tok[blockIdx.z] > 0 ? blockIdx.z : 1 - blockIdx.z;
-  const PlanLayout L = plan_layout(list, p.T, p.R, p.G, p.nkv, gridDim.x);
-  const int32_t* plan = p.plan + list_start(list, p.T, p.R, p.G, p.nkv, gridDim.x);
-  if (plan[0] != p.key) return;
-  const int part_rows = part_rows_of(list, p.T, p.R, p.G);
-  const size_t part0 = part_start(list, p.T, p.R, p.G, gridDim.x);
-  const int4* mg = reinterpret_cast<const int4*>(plan + L.merge) + 2 * (size_t)blockIdx.x;
-  const int4 a = mg[0], b = mg[1];  // row0, tokens, kv head, first CTA; slot of the first part, parts
-  const int lane = threadIdx.x & 31;
+  if (key != p.key) return;
   for (int rr = blockIdx.y * kMergeWarps + (threadIdx.x >> 5); rr < a.y * p.G; rr += gridDim.y * kMergeWarps) {
     const int tt = rr / p.G, qh = a.z * p.G + rr % p.G, row = a.x + tt;
     auto part = [&](int s) -> size_t { return part0 + (size_t)(s == 0 ? b.x : 2 * (a.w + s)) * part_rows + rr; };
     const float sink = p.sinks ? p.sinks[qh] * kLog2e : -INFINITY;
-    float M = sink;
-    for (int s = lane; s < b.y; s += 32) M = fmaxf(M, p.part_ml[part(s) * 2]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
-    float sum = p.sinks ? exp2f(sink - M) : 0.f, acc[VL];
+    // the parts in turn, the row's sum and output scaled to the largest maximum so far
+    float M = sink, sum = p.sinks ? 1.f : 0.f, acc[VL];
 #pragma unroll
     for (int k = 0; k < VL; ++k) acc[k] = 0.f;
-    for (int s0 = 0; s0 < b.y; s0 += 32) {
-      float w = 0.f, wl = 0.f;
-      if (s0 + lane < b.y) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + part(s0 + lane) * 2);
-        w = ml.x == -INFINITY ? 0.f : exp2f(ml.x - M);
-        wl = w * ml.y;
-      }
+    for (int s0 = 0; s0 < b.y; s0 += AHEAD) {
+      float2 ml[AHEAD], o[AHEAD][VL / 2];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) wl += __shfl_xor_sync(0xFFFFFFFFu, wl, o);
-      sum += wl;
-      const int e = min(32, b.y - s0);
-#pragma unroll 8
-      for (int s = 0; s < e; ++s) {
-        const float f = __shfl_sync(0xFFFFFFFFu, w, s);
-        const float2* src = reinterpret_cast<const float2*>(p.part_o + part(s0 + s) * DV + lane * VL);
+      for (int s = 0; s < AHEAD; ++s) {
+        ml[s] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int k = 0; k < VL / 2; ++k) o[s][k] = make_float2(0.f, 0.f);
+        if (s0 + s < b.y) {
+          const size_t at = part(s0 + s);
+          ml[s] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+#pragma unroll
+          for (int k = 0; k < VL / 2; ++k)
+            o[s][k] = reinterpret_cast<const float2*>(p.part_o + at * DV + lane * VL)[k];
+        }
+      }
+      float Mn = M;
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) Mn = fmaxf(Mn, ml[s].x);
+      const float f0 = M == -INFINITY ? 0.f : exp2f(M - Mn);
+      sum *= f0;
+#pragma unroll
+      for (int k = 0; k < VL; ++k) acc[k] *= f0;
+      M = Mn;
+#pragma unroll
+      for (int s = 0; s < AHEAD; ++s) {
+        const float f = ml[s].x == -INFINITY ? 0.f : exp2f(ml[s].x - M);
+        sum = fmaf(f, ml[s].y, sum);
 #pragma unroll
         for (int k = 0; k < VL / 2; ++k) {
-          const float2 o = src[k];
-          acc[2 * k] = fmaf(f, o.x, acc[2 * k]);
-          acc[2 * k + 1] = fmaf(f, o.y, acc[2 * k + 1]);
+          acc[2 * k] = fmaf(f, o[s][k].x, acc[2 * k]);
+          acc[2 * k + 1] = fmaf(f, o[s][k].y, acc[2 * k + 1]);
         }
       }
     }
@@ -1150,6 +1157,11 @@ template <int DQK, int DV>
 cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
   const Lists ls = lists_of(p.T, p.R, p.G);
   const bool both = ls.tok[kSmall] > 0 && ls.tok[kLarge] > 0;
+  for (int l : {kSmall, kLarge}) {
+    const PlanLayout L = plan_layout(l, p.T, p.R, p.G, p.nkv, num_sms);
+    p.list[l] = {list_start(l, p.T, p.R, p.G, p.nkv, num_sms), L.head, L.merge, L.segs,
+                 part_start(l, p.T, p.R, p.G, num_sms), part_rows_of(l, p.T, p.R, p.G)};
+  }
   cudaError_t e = cudaSuccess;
   if (ls.tok[kLarge] > 0) e = launch_list<DQK, DV, kLarge>(p, num_sms, st);
   if (e != cudaSuccess) return e;
@@ -1158,7 +1170,7 @@ cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const int rows = std::max(part_rows_of(kSmall, p.T, p.R, p.G), part_rows_of(kLarge, p.T, p.R, p.G));
   return launch_k(paged_attn_merge_kernel<DV>,
-                  dim3(num_sms, std::min(4, (rows + kMergeWarps - 1) / kMergeWarps), both ? 2 : 1),
+                  dim3(num_sms, std::min(8, (rows + kMergeWarps - 1) / kMergeWarps), both ? 2 : 1),
                   dim3(kMergeWarps * 32), 0, st, p);
 }
 
