@@ -17,8 +17,9 @@
 //                    when a row's maximum grows by more than 2^8 (P stays below 256);
 //   warps 8, 11      TMA producers of Q and K, and of V: chunks of 64 dims x 128 positions (16 KB) through one ring of
 //                    shared-memory slots, K_0 V_0 K_1 V_1 ...; a box is
-//                    64 dims of a page, and pages nobody sees are read as zeros from behind the pool's end.  Two warps,
-//                    because with pages of 16 tokens a block is 40 boxes;
+//                    64 dims of a page that some query of the unit sees.  A box takes its lane 125 cycles to issue, and
+//                    with pages of 16 tokens a block is 40: hence two warps (five, one for each chunk, were slower:
+//                    156 us against 118 for 64 decoding requests of 3500 tokens on average);
 //   warp 9           MMA issuer: S = Q K^T and O += P V, alternating the tiles, so that one tile's products
 //                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV and its
 //                    next S are issued in this order, so when that S is there, O holds PV and P is consumed;
@@ -489,14 +490,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     return;
   }
 
+  // a small unit's rows are all in the first warp of a tile
+  constexpr int kRowThreads = LIST == kSmall ? 32 : 128;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < NG; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < NG; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 128);
+      mbar_init(&p_full[i], kRowThreads);
       mbar_init(&o_full[i], 1);
     }
     mbar_init(fix_req, 1);
@@ -543,87 +549,96 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   } list{segs, first_a, first_b, nseg};
   bool ok = true;
 
+  // TMA producer of Q and K, or of V.  One lane issues: a box takes it some 125 cycles.  Pages that no query sees are left
+  // out.
+  auto produce = [&](bool isv) {
+    const int c0 = isv ? S::QCH : 0, c1 = isv ? CPB : S::QCH;
+    const CUtensorMap* map = isv ? &p.vmap : &p.kmap;
+    if (lane == 0) {
+      tma_prefetch_map(map);
+      if (!isv) tma_prefetch_map(&p.qmap);
+    }
+    const int P = 1 << p.page_shift, ppb = 128 >> p.page_shift;  // pages per block
+    const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
+    uint32_t ci = c0, nb = 0;                                    // ring chunk, key blocks issued
+    uint32_t freed = 0;                                          // ring blocks known to be free again
+    uint32_t nq = 0, turn = 0;                                   // phases of the Q buffers, the next single tile's
+    for (int s = 0; s < nseg && ok; ++s) {
+      const Seg g = list.next();
+      const int qlast = g.qfirst + g.ntok - 1;
+      const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
+      const int* trow = p.table + (size_t)g.r * p.width;
+      // the number of the block's page `lane`, num_pages for one nobody sees; loaded a block ahead
+      auto page_of = [&](int j) -> int {
+        const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb);
+        const int pg = kb * ppb + lane, pos = pg << p.page_shift;
+        if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return p.num_pages;
+        return trow[pg];
+      };
+      int page = page_of(g.b0);
+      for (int j = 0; j < g.nblk && ok; ++j) {
+        int row = nowhere;
+        if ((unsigned)page < (unsigned)p.num_pages) row = page * p.nkv + g.hk;
+        else if (page != p.num_pages) set_status(p.status, MIMO_ERANGE);
+        const uint32_t seen = __ballot_sync(0xFFFFFFFFu, page != p.num_pages);
+        if (j + 1 < g.nblk) page = page_of(g.b0 + j + 1);
+        int rows[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, row, i);
+        uint64_t* bar = &full[(2 * nb + (isv ? 1 : 0)) % NG];
+        for (int c = c0; c < c1; ++c) {
+          const uint32_t at = ci + (c - c0);
+          if (at >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
+            const uint32_t old = at - NS, of = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
+            if (ok && of >= freed) ok = mbar_wait(&empty[of % NG], (of / NG) & 1);
+            freed = of + 1;
+          }
+          ok = __all_sync(0xFFFFFFFFu, ok);
+          if (!ok) break;
+          if (lane == 0) {
+            if (c == c0) mbar_arrive_expect_tx(bar, (uint32_t)((c1 - c0) * __popc(seen) * P * 128));
+            uint8_t* dst = sRing + (at % NS) * kChunk;
+            const int dim = (isv ? c - S::QCH : c) * 64;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if ((seen >> i) & 1) tma_box(dst + i * P * 128, map, dim, 0, rows[i], bar);
+          }
+          __syncwarp();
+        }
+        if (!isv && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
+          const bool pair = LIST == kLarge && g.ntok > tpt;
+          for (int x = 0; x < (pair ? 2 : 1); ++x) {
+            const int qb = pair ? x : turn;
+            if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
+            nq ^= 1u << qb;
+            if (lane == 0 && ok) {
+              mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
+#pragma unroll
+              for (int d = 0; d < S::QCH; ++d)
+                tma_box(sQ + qb * S::QB + d * S::QCHUNK, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[qb]);
+            }
+          }
+          if (!pair) turn ^= 1;
+        }
+        ci += CPB;
+        ++nb;
+      }
+    }
+    // no copy may still be landing when the CTA exits: the last blocks (after a wait that ran out, what there is of the
+    // block it was in: this wait runs out too), and Q
+    const uint32_t begun = ok ? nb : nb + 1;
+    for (uint32_t k = 0; k < (uint32_t)NG / 2 && k < begun; ++k) {
+      const uint32_t i = 2 * (begun - 1 - k) + (isv ? 1 : 0);
+      mbar_wait(&full[i % NG], (i / NG) & 1);
+    }
+    if (!isv)
+      for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
+  };
+
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
-    if (warp == 8 || warp == 11) {  // ------------------------------------------------- TMA producers: Q and K, V
-      const bool isv = warp == 11;
-      const CUtensorMap* map = isv ? &p.vmap : &p.kmap;
-      const int chunks = isv ? S::VCH : S::QCH;
-      if (lane == 0) {
-        tma_prefetch_map(map);
-        if (!isv) tma_prefetch_map(&p.qmap);
-      }
-      const int P = 1 << p.page_shift, ppb = 128 >> p.page_shift;  // pages per block
-      const int nowhere = p.num_pages * p.nkv;                    // a row of pages behind the pool: reads zeros
-      uint32_t ci = isv ? S::QCH : 0, nb = 0;                      // ring chunk, key blocks issued
-      uint32_t freed = 0;                                          // ring blocks known to be free again
-      uint32_t nq = 0, turn = 0;                                   // phases of the Q buffers, the next single tile's
-      for (int s = 0; s < nseg && ok; ++s) {
-        const Seg g = list.next();
-        const int qlast = g.qfirst + g.ntok - 1;
-        const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
-        const int* trow = p.table + (size_t)g.r * p.width;
-        // the number of the block's page `lane`, num_pages for one nobody sees; loaded a block ahead
-        auto page_of = [&](int j) -> int {
-          const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb);
-          const int pg = kb * ppb + lane, pos = pg << p.page_shift;
-          if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return p.num_pages;
-          return trow[pg];
-        };
-        int page = page_of(g.b0);
-        for (int j = 0; j < g.nblk && ok; ++j) {
-          int row = nowhere;
-          if ((unsigned)page < (unsigned)p.num_pages) row = page * p.nkv + g.hk;
-          else if (page != p.num_pages) set_status(p.status, MIMO_ERANGE);
-          if (j + 1 < g.nblk) page = page_of(g.b0 + j + 1);
-          int rows[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, row, i);
-          uint64_t* bar = &full[(2 * nb + (isv ? 1 : 0)) % NG];
-          for (int c = 0; c < chunks; ++c) {
-            if (ci + c >= (uint32_t)NS) {  // the ring block whose chunk was in this slot must have been read
-              const uint32_t old = ci + c - NS, of = 2 * (old / CPB) + (old % CPB >= (uint32_t)S::QCH ? 1 : 0);
-              if (ok && of >= freed) ok = mbar_wait(&empty[of % NG], (of / NG) & 1);
-              freed = of + 1;
-            }
-            ok = __all_sync(0xFFFFFFFFu, ok);
-            if (!ok) break;
-            if (lane == 0) {
-              if (c == 0) mbar_arrive_expect_tx(bar, chunks * kChunk);
-              uint8_t* dst = sRing + ((ci + c) % NS) * kChunk;
-#pragma unroll
-              for (int i = 0; i < 8; ++i)
-                if (i < ppb) tma_box(dst + i * P * 128, map, c * 64, 0, rows[i], bar);
-            }
-            __syncwarp();
-          }
-          if (!isv && j == 0) {  // Q behind the first K block: both buffers, or the one whose turn it is
-            const bool pair = LIST == kLarge && g.ntok > tpt;
-            for (int x = 0; x < (pair ? 2 : 1); ++x) {
-              const int qb = pair ? x : turn;
-              if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
-              nq ^= 1u << qb;
-              if (lane == 0 && ok) {
-                mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
-#pragma unroll
-                for (int d = 0; d < S::QCH; ++d)
-                  tma_box(sQ + qb * S::QB + d * S::QCHUNK, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[qb]);
-              }
-            }
-            if (!pair) turn ^= 1;
-          }
-          ci += CPB;
-          ++nb;
-        }
-      }
-      // no copy may still be landing when the CTA exits: the last blocks (after a wait that ran out, what there is of
-      // the block it was in: this wait runs out too), and Q
-      for (uint32_t k = 0; k < (uint32_t)NG / 2 && k < nb; ++k) {
-        const uint32_t i = 2 * (nb - 1 - k) + (isv ? 1 : 0);
-        mbar_wait(&full[i % NG], (i / NG) & 1);
-      }
-      if (!isv)
-        for (int x = 0; x < 2; ++x) mbar_wait(&q_full[x], ((nq >> x) & 1) ^ 1);
+    if (warp == 8 || warp == 11) {
+      produce(warp == 11);
     } else if (warp == 9) {
       // --------------------------------------------------------------------------------------------- MMA issuer
       // The whole warp runs this and one elected lane issues: what all lanes agree on stays in uniform registers, which
@@ -784,7 +799,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           ok = mbar_wait(fix_req, fixes++ & 1);  // the block's V is there
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
-          // pages nobody sees hold zeros already; what is left are rows of the pages at the ends of what is seen
           auto zero = [&](int from, int to) {
             from = max(from, kp), to = min(to, kp + 128);
             for (int i = from * 8 + lane; i < to * 8; i += 32) {  // a row is 128 bytes whatever the swizzle
@@ -794,10 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
                     make_uint4(0, 0, 0, 0);
             }
           };
-          const int in_page = (1 << p.page_shift) - 1;
-          zero(qlast + 1, (qlast | in_page) + 1);
-          zero(max(bl.lo & ~in_page, bl.keep), bl.lo);
-          if (bl.keep > 0) zero(bl.keep, min((bl.keep - 1 | in_page) + 1, bl.lo));
+          zero(qlast + 1, kp + 128);
+          zero(bl.keep, bl.lo);
           tc::fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) mbar_arrive(v_fixed);
@@ -807,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   } else {  // ------------------------------------------------------------------------------- softmax of tile x
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(kRegsSoftmax));
     const int x = warp >> 2, r = threadIdx.x & 127;
+    if (LIST != kSmall || (warp & 3) == 0) {  // a small unit's rows are a tile's first warp's
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t tS = tbase + x * 128 + lane_off, tO = tbase + 256 + x * DV + lane_off;
     const int head = r % p.G;  // this row's head of the group
@@ -953,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       bool own = true, other = false;  // whether there is such an output (one never written may hold anything)
       if (!pair) {
         xchg[x * 128 + r] = make_float2(m_ref, l);
-        named_bar_sync(1, 256);
+        named_bar_sync(1, 2 * kRowThreads);
         const float2 o = xchg[(x ^ 1) * 128 + r];
         const float M = fmaxf(m_ref, o.x);
         own = m_ref != -INFINITY || l != 0.f, other = o.x != -INFINITY || o.y != 0.f;
@@ -1053,7 +1066,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         if (store && g.slot >= 0 && c0 == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
       }
       tc::tc_fence_before();
-      if (!pair) named_bar_sync(2, 256);  // both outputs are read, and the exchange may be written again
+      if (!pair) named_bar_sync(2, 2 * kRowThreads);  // both outputs are read, and the exchange may be written again
+    }
     }
   }
   if (!ok && p.status) set_status(p.status, MIMO_ETIMEOUT);
