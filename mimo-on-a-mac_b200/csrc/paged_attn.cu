@@ -27,7 +27,6 @@
 //                    hold anything, and 0 * NaN is not 0.
 // Every wait is bounded and sets MIMO_ETIMEOUT; the producer drains its copies and the issuer its MMAs before exit.
 #include <cstring>
-#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -329,6 +328,11 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
 __device__ __forceinline__ float ex2_approx(float x) {  // 2^x on the special-function unit: 2^-inf = +0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {  // within an ulp
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t pack_bf16x2_rn(float lo, float hi) {
@@ -839,6 +843,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       float m_ref = -INFINITY, m_new = -INFINITY, l = 0.f;
       bool fresh = true;
       const float sink = p.sinks && row_ok ? p.sinks[g.hk * p.G + head] * kLog2e : 0.f;
+      // where the row's output goes, worked out while the scores are on their way: itself, or a part in the workspace;
+      // and the rows of the quad's lanes, which exchange theirs
+      const int row = g.row0 + tt;
+      const bool store = row_ok && row < p.T;
+      const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
+      uint8_t* to = g.slot < 0 ? reinterpret_cast<uint8_t*>(p.out + ((size_t)row * p.nq + g.hk * p.G + head) * DV)
+                               : reinterpret_cast<uint8_t*>(p.part_o + at * DV);
+      uint8_t* quad_to[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        quad_to[k] = reinterpret_cast<uint8_t*>(
+            __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(to), (lane & ~3) | k));
+      const uint32_t quad_ok = __ballot_sync(0xFFFFFFFFu, store) >> (lane & ~3);
       // after a wait that ran out the loops go on without work, for the barriers that both groups must pass
       for (int j = pair ? 0 : x; j < g.nblk; j += pair ? 1 : 2) {
         if (ok) ok = mbar_wait(&s_full[x], ns & 1);
@@ -970,46 +987,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         const float2 o = xchg[(x ^ 1) * 128 + r];
         const float M = fmaxf(m_ref, o.x);
         own = m_ref != -INFINITY || l != 0.f, other = o.x != -INFINITY || o.y != 0.f;
-        w_own = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
-        w_other = o.x == -INFINITY ? 0.f : exp2f(o.x - M);
+        w_own = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - M);
+        w_other = o.x == -INFINITY ? 0.f : ex2_approx(o.x - M);
         l = l * w_own + o.y * w_other;
         m_ref = M;
         c0 = x * (DV / 2), c1 = c0 + DV / 2;
       }
       tc::tc_fence_after();
       if (work && ok) {
-        const int qh = g.hk * p.G + head, row = g.row0 + tt;
         const uint32_t tOther = tbase + 256 + (x ^ 1) * DV + lane_off;
         float f = 1.f;  // an unnormalised part: maximum (log2), sum and output of these blocks
         if (g.slot < 0) {
           if (p.sinks) {
             const float M = fmaxf(m_ref, sink);
-            const float a = m_ref == -INFINITY ? 0.f : exp2f(m_ref - M);
-            f = a / (l * a + exp2f(sink - M));
+            const float a = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - M);
+            f = a * rcp_approx(l * a + ex2_approx(sink - M));
           } else {
-            f = l == 0.f ? 0.f : 1.f / l;
+            f = l == 0.f ? 0.f : rcp_approx(l);
           }
         }
         w_own *= f, w_other *= f;
-        const bool store = row_ok && row < p.T;
-        const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
-        // N columns from c on: scaled, joined, written
-        auto emit = [&](auto n, int c) {
-          constexpr int N = decltype(n)::value;
-          float o[N];
-#pragma unroll
-          for (int k = 0; k < N; k += 32) tmem_ld32(tO + c + k, o + k);
+#pragma unroll 1
+        for (int c = c0; c < c1; c += 32) {
+          float o[32];
+          tmem_ld32(tO + c, o);
           if (pair) {
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < N; ++e) o[e] *= w_own;
+            for (int e = 0; e < 32; ++e) o[e] *= w_own;
           } else {
-            float q[N];
-#pragma unroll
-            for (int k = 0; k < N; k += 32) tmem_ld32(tOther + c + k, q + k);
+            float q[32];
+            tmem_ld32(tOther + c, q);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
+            for (int e = 0; e < 32; ++e) {
               o[e] = own ? o[e] * w_own : 0.f;
               o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
             }
@@ -1017,51 +1028,37 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           if (g.slot >= 0) {
             if (store)
 #pragma unroll
-              for (int e = 0; e < N; e += 8) st_global_v8(p.part_o + at * DV + c + e, reinterpret_cast<uint32_t*>(o + e));
-            return;
+              for (int e = 0; e < 32; e += 8)
+                st_global_v8(reinterpret_cast<float*>(to) + c + e, reinterpret_cast<uint32_t*>(o + e));
+            continue;
           }
-          uint32_t w[N / 2];
+          // The 32 columns are 64 bytes of a row.  A store of a piece of 32 different rows takes the load/store unit 32
+          // turns, so the four lanes of a quad first exchange theirs: the 16 bytes q of the quad's rows go to lane q, and a
+          // store writes 64 bytes of 8 rows.
+          uint32_t w[16];
 #pragma unroll
-          for (int e = 0; e < N / 2; ++e) w[e] = pack_bf16x2_rn(o[2 * e], o[2 * e + 1]);
-          uint16_t* dst = p.out + ((size_t)row * p.nq + qh) * DV + c;
-          if constexpr (N == 64) {
-            // A row is 128 bytes here.  A store of one piece of 32 different rows takes the load/store unit 32 turns (a
-            // unit's 128 x 128 outputs took 7600 cycles that way), so the four lanes of a quad first exchange theirs:
-            // chunk q (32 bytes) of the quad's rows goes to lane q, and a store writes whole rows.
-            const int q = lane & 3;
+          for (int e = 0; e < 16; ++e) w[e] = pack_bf16x2_rn(o[2 * e], o[2 * e + 1]);
 #pragma unroll
-            for (int st = 0; st < 2; ++st) {
-              const bool hi = (q >> st) & 1;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if ((k >> st) & 1) continue;
-                const int k1 = k | (1 << st);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  const uint32_t give = hi ? w[k * 8 + e] : w[k1 * 8 + e];
-                  const uint32_t take = __shfl_xor_sync(0xFFFFFFFFu, give, 1 << st);
-                  w[k * 8 + e] = hi ? take : w[k * 8 + e];
-                  w[k1 * 8 + e] = hi ? w[k1 * 8 + e] : take;
-                }
-              }
-            }
+          for (int st = 0; st < 2; ++st) {
+            const bool hi = (lane >> st) & 1;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              const bool yes = __shfl_sync(0xFFFFFFFFu, (int)store, (lane & ~3) | k) != 0;
-              uint16_t* to = reinterpret_cast<uint16_t*>(
-                  __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(dst), (lane & ~3) | k));
-              if (yes) st_global_v8(to + q * 16, w + k * 8);
-            }
-          } else if (store) {
+              if ((k >> st) & 1) continue;
+              const int k1 = k | (1 << st);
 #pragma unroll
-            for (int e = 0; e < N / 2; e += 8) st_global_v8(dst + e * 2, w + e);
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t give = hi ? w[k * 4 + e] : w[k1 * 4 + e];
+                const uint32_t take = __shfl_xor_sync(0xFFFFFFFFu, give, 1 << st);
+                w[k * 4 + e] = hi ? take : w[k * 4 + e];
+                w[k1 * 4 + e] = hi ? w[k1 * 4 + e] : take;
+              }
+            }
           }
-        };
-        if (DV == 64 && !pair) {
-          emit(std::integral_constant<int, 32>{}, c0);
-        } else {
-#pragma unroll 1
-          for (int c = c0; c < c1; c += 64) emit(std::integral_constant<int, 64>{}, c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if ((quad_ok >> k) & 1)
+              *reinterpret_cast<uint4*>(quad_to[k] + c * 2 + (lane & 3) * 16) =
+                  make_uint4(w[k * 4], w[k * 4 + 1], w[k * 4 + 2], w[k * 4 + 3]);
         }
         if (store && g.slot >= 0 && c0 == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
       }
