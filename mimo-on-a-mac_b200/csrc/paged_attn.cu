@@ -17,9 +17,8 @@
 //                    when a row's maximum grows by more than 2^8 (P stays below 256);
 //   warps 8, 11      TMA producers of Q and K, and of V: chunks of 64 dims x 128 positions (16 KB) through one ring of
 //                    shared-memory slots, K_0 V_0 K_1 V_1 ...; a box is
-//                    64 dims of a page that some query of the unit sees.  A box takes its lane 125 cycles to issue, and
-//                    with pages of 16 tokens a block is 40: hence two warps (five, one for each chunk, were slower:
-//                    156 us against 118 for 64 decoding requests of 3500 tokens on average);
+//                    64 dims of a page that some query of the unit sees.  With pages of 16 tokens a block is 40
+//                    boxes: hence two warps;
 //   warp 9           MMA issuer: S = Q K^T and O += P V, alternating the tiles, so that one tile's products
 //                    run while the other's softmax does: S_A S_B | PV_A S_A' | PV_B S_B' | ...  A tile's PV and its
 //                    next S are issued in this order, so when that S is there, O holds PV and P is consumed;
@@ -27,6 +26,7 @@
 //                    hold anything, and 0 * NaN is not 0.
 // Every wait is bounded and sets MIMO_ETIMEOUT; the producer drains its copies and the issuer its MMAs before exit.
 #include <cstring>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -553,10 +553,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   } list{segs, first_a, first_b, nseg};
   bool ok = true;
 
-  // TMA producer of Q and K, or of V.  One lane issues: a box takes it some 125 cycles.  Pages that no query sees are left
-  // out.
-  auto produce = [&](bool isv) {
-    const int c0 = isv ? S::QCH : 0, c1 = isv ? CPB : S::QCH;
+  // TMA producer of Q and K, or of V.  The whole warp runs it and an elected lane issues: a copy then takes 25 cycles to
+  // issue, where a branch of lane 0 took 74 alone and 125 here (a block of pages of 16 tokens is 40 copies).  Pages that no
+  // query sees are left out.
+  auto produce = [&](auto of_v) {
+    constexpr bool isv = decltype(of_v)::value;
+    constexpr int c0 = isv ? S::QCH : 0, c1 = isv ? CPB : S::QCH;
     const CUtensorMap* map = isv ? &p.vmap : &p.kmap;
     if (lane == 0) {
       tma_prefetch_map(map);
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         else if (page != p.num_pages) set_status(p.status, MIMO_ERANGE);
         const uint32_t seen = __ballot_sync(0xFFFFFFFFu, page != p.num_pages);
         if (j + 1 < g.nblk) page = page_of(g.b0 + j + 1);
-        int rows[8];
+        int rows[8];  // the same in all lanes: uniform registers, from which a copy is issued in 25 cycles
 #pragma unroll
         for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, row, i);
         uint64_t* bar = &full[(2 * nb + (isv ? 1 : 0)) % NG];
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           }
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
-          if (lane == 0) {
+          if (elect_one()) {
             if (c == c0) mbar_arrive_expect_tx(bar, (uint32_t)((c1 - c0) * __popc(seen) * P * 128));
             uint8_t* dst = sRing + (at % NS) * kChunk;
             const int dim = (isv ? c - S::QCH : c) * 64;
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
             const int qb = pair ? x : turn;
             if (ok) ok = mbar_wait(&q_empty[qb], ((nq >> qb) & 1) ^ 1);
             nq ^= 1u << qb;
-            if (lane == 0 && ok) {
+            if (ok && elect_one()) {
               mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
 #pragma unroll
               for (int d = 0; d < S::QCH; ++d)
@@ -641,8 +643,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(kRegsOther));
-    if (warp == 8 || warp == 11) {
-      produce(warp == 11);
+    if (warp == 8) {
+      produce(std::false_type{});
+    } else if (warp == 11) {
+      produce(std::true_type{});
     } else if (warp == 9) {
       // --------------------------------------------------------------------------------------------- MMA issuer
       // The whole warp runs this and one elected lane issues: what all lanes agree on stays in uniform registers, which
@@ -883,32 +887,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               }
             }
           };
-          // A new reference: O, which holds the products of the blocks before (see above), and the sum are scaled to it.
-          auto refer = [&](float to, bool mine) {
-            const float alpha = mine && m_ref != -INFINITY ? ex2_approx(m_ref - to) : 1.f;
-            if (mine) m_ref = to;
-            l *= alpha;
-            if (!__any_sync(0xFFFFFFFFu, alpha != 1.f)) return;
-#pragma unroll 1
-            for (int c = 0; c < DV; c += 16) {
-              float o[16];
-              tc::tmem_ld<16>(tO + c, o);
-              tc::tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] *= alpha;
-              tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
-            }
-            tmem_wait_st();
-          };
           // The reference of the exponentials is a maximum of what came before: a bf16 or float32 value is as exact beside
           // 2^60 as beside 1, so the exponentials need not wait for their own maximum.  A maximum 2^8 above the reference
           // is taken up at the next block, one 2^60 above it (and a row's first) at once.
           // (rows without a query have no say: what they compute on may be anything)
-          const bool later = row_ok && m_new > m_ref + 8.f;
-          if (__any_sync(0xFFFFFFFFu, later)) refer(m_new, later);
+          float to = m_new;
+          bool now = row_ok && m_new > m_ref + 8.f;
           m_new = -INFINITY;
-          // The halves one after the other through the same instructions: written out for both, with the rare repetition,
-          // the loop was larger than the instruction caches hold, and the warps waited for it.
+          // The halves one after the other through the same instructions, and one copy of what is rare: written out, the
+          // loop was larger than the instruction caches hold, and the warps waited for it.
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {
             float v[64];
@@ -921,12 +908,44 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
 #pragma unroll
               for (int e = 1; e < 63; e += 2) a = fmaxf(fmaxf(a, v[e]), v[e + 1]);
               a = fmaxf(a, v[63]) * sl2;
-              refer(a, row_ok && m_ref == -INFINITY && a > -INFINITY);
-              fresh = __any_sync(0xFFFFFFFFu, row_ok && m_ref == -INFINITY);
+              if (row_ok && m_ref == -INFINITY && a > -INFINITY) to = a, now = true;
             }
             uint32_t pk[32];
             uint64_t sum[2];
+            bool again = false;  // the half's exponentials once more
             for (;;) {
+              // A new reference: O, which holds the products of the blocks before (see above), the sum, and in a second
+              // half the first half's P are scaled to it.
+              if (__any_sync(0xFFFFFFFFu, now)) {
+                const float alpha = now && m_ref != -INFINITY ? ex2_approx(m_ref - to) : 1.f;
+                if (now) m_ref = to;
+                l *= alpha;
+                if (__any_sync(0xFFFFFFFFu, alpha != 1.f)) {
+#pragma unroll 1
+                  for (int c = 0; c < DV; c += 16) {
+                    float o[16];
+                    tc::tmem_ld<16>(tO + c, o);
+                    tc::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] *= alpha;
+                    tmem_st16(tO + c, reinterpret_cast<const uint32_t*>(o));
+                  }
+                  tmem_wait_st();
+                  if (again && hf == 1) {
+#pragma unroll 1
+                    for (int c = 0; c < 32; ++c) {
+                      float w[1];
+                      tc::tmem_ld<1>(tS + c, w);
+                      tc::tmem_wait_ld();
+                      const uint32_t u = __float_as_uint(w[0]);
+                      tmem_st1(tS + c, pack_bf16x2_rn(__uint_as_float(u << 16) * alpha,
+                                                      __uint_as_float(u & 0xFFFF0000u) * alpha));
+                    }
+                    tmem_wait_st();
+                  }
+                }
+                fresh = __any_sync(0xFFFFFFFFu, row_ok && m_ref == -INFINITY);
+              }
               // P = bf16(2^(s * scale * log2 e - reference)) and their sum, and their maximum on the way (the scale is
               // positive, so it orders the scaled scores alike).  The special-function unit bounds this loop, and what
               // else it does has to lie between its instructions.
@@ -942,28 +961,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
                 sum[i & 1] = add2(sum[i & 1], pack2(p0, p1));
                 pk[i] = pack_bf16x2_rn(p0, p1);  // rounded to bf16 for the product with V, the sum is not
               }
-              const float m = fmaxf(a, b) * sl2;
-              const bool jump = row_ok && m > m_ref + 60.f;
-              m_new = fmaxf(m_new, m);
-              if (!__any_sync(0xFFFFFFFFu, jump)) break;
-              const float was = m_ref;
-              refer(m, jump);
-              if (hf == 1) {  // the first half's P as well
-                const float alpha = jump && was != -INFINITY ? ex2_approx(was - m) : 1.f;
-                tmem_wait_st();
-#pragma unroll 1
-                for (int c = 0; c < 32; c += 8) {
-                  float w[8];
-                  tc::tmem_ld<8>(tS + c, w);
-                  tc::tmem_wait_ld();
-#pragma unroll
-                  for (int e = 0; e < 8; ++e) {
-                    const uint32_t u = __float_as_uint(w[e]);
-                    const uint32_t z = pack_bf16x2_rn(__uint_as_float(u << 16) * alpha, __uint_as_float(u & 0xFFFF0000u) * alpha);
-                    tmem_st1(tS + c + e, z);
-                  }
-                }
-              }
+              to = fmaxf(a, b) * sl2;
+              m_new = fmaxf(m_new, to);
+              now = row_ok && to > m_ref + 60.f;
+              again = __any_sync(0xFFFFFFFFu, now);
+              if (!again) break;
             }
             const float2 s0 = unpack2(add2(sum[0], sum[1]));
             l += s0.x + s0.y;
