@@ -346,12 +346,16 @@ class DecoderStack:
                 h, r = add_rmsnorm(hh, y, nxt.input_norm, nxt.eps)
             else:
                 h = add(hh, y)
+        out = self._result(h)
+        out.copy_(h)
+        return out
+
+    def _result(self, h: torch.Tensor) -> torch.Tensor:
+        """The fixed output buffer of h's shape."""
         key = (tuple(h.shape), h.device)
         if key not in self._out:
             self._out[key] = torch.empty_like(h)
-        out = self._out[key]
-        out.copy_(h)
-        return out
+        return self._out[key]
 
 
 def synthetic_attention(cfg: AttentionConfig, hidden: int = 4096, seed: int = 4, std: float = 0.02,

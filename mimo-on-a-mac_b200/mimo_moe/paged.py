@@ -75,7 +75,7 @@ def _page_size(page_size: int) -> int:
 
 class PageStep:
     """The row layout of one step of R requests (what page_plan writes; a program with a page allocator of its own
-    fills it itself): block_table int32 [R, width], cu_q int32 [R + 1], seq_lens int32 [R] (lengths with the step's
+    fills it itself, with a slot of its own for every row): block_table int32 [R, width], cu_q int32 [R + 1], seq_lens int32 [R] (lengths with the step's
     tokens), positions and slots int32 [tokens].  n_free int32 [1] and status int32 [1] are page_plan's."""
 
     def __init__(self, *, block_table: torch.Tensor, page_size: int, cu_q: torch.Tensor, seq_lens: torch.Tensor,
@@ -100,6 +100,7 @@ class PageStep:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else _int32(status, "status",
                                                                                                  (1,), dev)
         self.requests, self.width, self.tokens, self.device = R, block_table.shape[1], T, dev
+        self.rows = _Rows()   # scratch of the layers that work on this step, one after another
 
     @classmethod
     def empty(cls, requests: int, tokens: int, block_table: torch.Tensor, page_size: int,
@@ -109,14 +110,12 @@ class PageStep:
         if tokens < 0:
             raise ValueError(f"a step has no {tokens} token rows")
         dev = block_table.device
-        state = torch.zeros(requests + 1, dtype=torch.int32, device=dev)   # seq_lens | n_free
-        step = cls(block_table=block_table, page_size=page_size,
-                   cu_q=torch.zeros(requests + 1, dtype=torch.int32, device=dev), seq_lens=state[:requests],
+        return cls(block_table=block_table, page_size=page_size,
+                   cu_q=torch.zeros(requests + 1, dtype=torch.int32, device=dev),
+                   seq_lens=torch.zeros(requests, dtype=torch.int32, device=dev),
                    positions=torch.full((tokens,), -1, dtype=torch.int32, device=dev),
-                   slots=torch.full((tokens,), -1, dtype=torch.int32, device=dev), n_free=state[requests:],
-                   status=status)
-        step.state = state
-        return step
+                   slots=torch.full((tokens,), -1, dtype=torch.int32, device=dev),
+                   n_free=torch.zeros(1, dtype=torch.int32, device=dev), status=status)
 
     def last_rows(self) -> torch.Tensor:
         """The row of each request's last new token, int32 [R] (the rows whose hidden state goes to the lm_head); a
@@ -181,6 +180,23 @@ def page_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Tens
               "page_release")
 
 
+class _Rows:
+    """Buffers with a row for each token of a step, grown as steps of more rows come.  A buffer that was outgrown is
+    kept: a captured graph may hold its address."""
+
+    def __init__(self):
+        self._bufs, self._outgrown = {}, []
+
+    def get(self, key, rows: int, make) -> torch.Tensor:
+        """The first `rows` rows of the buffer `key`; make(n) makes one of n rows."""
+        buf = self._bufs.get(key)
+        if buf is None or buf.shape[0] < rows:
+            if buf is not None:
+                self._outgrown.append(buf)
+            buf = self._bufs[key] = make(max(rows, 2 * buf.shape[0] if buf is not None else rows))
+        return buf[:rows]
+
+
 class PageTable:
     """Block tables, lengths and free pages of up to max_requests requests of at most max_len tokens, over pools of
     num_pages pages.  Row r of every tensor is request r; a free row has length 0."""
@@ -201,17 +217,26 @@ class PageTable:
         self.lens, self.n_free = self._state[:max_requests], self._state[max_requests:]
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.requests, self.device = int(max_requests), self.block_table.device
-        self._steps = {}
+        self._cu_q = torch.zeros(max_requests + 1, dtype=torch.int32, device=dev)
+        self._after = torch.zeros(max_requests + 1, dtype=torch.int32, device=dev)   # the step's lengths and free pages
+        self._rows = _Rows()
 
     def step(self, new_lens: torch.Tensor, tokens: int) -> PageStep:
-        """Plan a step (page_plan) and take its lengths and free pages over.  The step's buffers are the table's, one
-        set for each row count, and the next step of that row count writes them again."""
-        out = self._steps.get(tokens)
-        if out is None:
-            out = self._steps[tokens] = PageStep.empty(self.requests, tokens, self.block_table, self.page_size,
-                                                       self.status)
+        """Plan a step (page_plan) and take its lengths and free pages over.  The step's buffers are the table's: the next
+        step writes them again."""
+        if tokens < 0:
+            raise ValueError(f"a step has no {tokens} token rows")
+        R = self.requests
+
+        def rows(n):
+            return torch.empty(n, dtype=torch.int32, device=self.device)
+
+        out = PageStep(block_table=self.block_table, page_size=self.page_size, cu_q=self._cu_q,
+                       seq_lens=self._after[:R], positions=self._rows.get("positions", tokens, rows),
+                       slots=self._rows.get("slots", tokens, rows), n_free=self._after[R:], status=self.status)
+        out.rows = self._rows
         page_plan(self.lens, new_lens, self.block_table, self.free_pages, self.n_free, self.page_size, tokens, out=out)
-        self._state.copy_(out.state)
+        self._state.copy_(self._after)
         return out
 
     def release(self, done: torch.Tensor) -> None:
@@ -241,19 +266,21 @@ class PagedKVCache:
         self.device = k.device
         self.step: Optional[PageStep] = None
         self.plan: Optional["AttentionPlan"] = None
-        self._out = {}
 
     def attend(self, qkv: torch.Tensor, sinks: Optional[torch.Tensor]) -> torch.Tensor:
-        """The layer's cache half (RoPE + append, attention) for the projection rows of `step`'s tokens.  Padding rows
-        of the result hold zeros or an earlier call's values: finite, and nothing anyone asks for."""
+        """The layer's cache half (RoPE + append, attention) for the projection rows of `step`'s tokens.  The result is
+        the step's scratch, which the next layer's call writes again; its padding rows hold zeros or an earlier call's
+        values: finite, and nothing anyone asks for."""
         step, cfg = self.step, self.cfg
         if step is None:
             raise ValueError("PagedKVCache: no step set (cache.step = table.step(new_lens, tokens))")
-        shape = (step.tokens, cfg.n_heads, cfg.v_head_dim)
-        if shape not in self._out:
-            self._out[shape] = torch.zeros(shape, dtype=torch.bfloat16, device=self.device)
+
+        def rows(n):
+            return torch.zeros(n, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=self.device)
+
+        out = step.rows.get(("attention", cfg.n_heads, cfg.v_head_dim), step.tokens, rows)
         q = rope_store_paged(qkv, cfg, self, step)
-        return attention_paged(q, self, cfg, step, sinks, plan=self.plan, out=self._out[shape])
+        return attention_paged(q, self, cfg, step, sinks, plan=self.plan, out=out)
 
 
 def _fits(cache: PagedKVCache, cfg: AttentionConfig, step: PageStep, where: str) -> None:
@@ -371,9 +398,10 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
 
 class PagedDecoderStack(DecoderStack):
     """DecoderStack for many requests: one PageTable and a PagedKVCache per layer.  __call__(x bf16 [tokens, hidden],
-    new_lens int32 [max_requests]) plans the step, runs the layers and returns a fixed buffer per shape; the lengths
-    advance on the device, so a decode step captured once as a CUDA graph serves the tokens that follow as well.
-    `release(done)` frees finished requests' rows.  Padding rows of x need only be finite."""
+    new_lens int32 [max_requests]) plans the step, runs the layers and returns the rows' hidden states (a buffer of the
+    stack's, which the next call writes again); the lengths advance on the device, so a decode step captured once as a
+    CUDA graph serves the tokens that follow as well.  `release(done)` frees finished requests' rows; `check()` raises
+    when a step could not be planned (it then ran without new tokens).  Padding rows of x need only be finite."""
 
     def __init__(self, layers, max_requests: int, max_len: int, num_pages: int, page_size: int = 64):
         if not layers:
@@ -382,7 +410,6 @@ class PagedDecoderStack(DecoderStack):
         dev = self.layers[0].attn.w_o.device
         self.table = PageTable(max_requests, max_len, num_pages, page_size, dev)
         self.caches = [PagedKVCache(l.attn.cfg, num_pages, page_size, dev) for l in self.layers]
-        self._out = {}
 
     def at(self, pos: int) -> "PagedDecoderStack":
         raise ValueError("a paged stack has a position for every request: table.lens")
@@ -393,6 +420,17 @@ class PagedDecoderStack(DecoderStack):
 
     def release(self, done: torch.Tensor) -> None:
         self.table.release(done)
+
+    def check(self) -> None:
+        """Synchronise on the status word of the table's steps (PageStep.check)."""
+        try:
+            read_status(self.table.status, "paged stack")
+        finally:
+            self.table.status.zero_()
+
+    def _result(self, h: torch.Tensor) -> torch.Tensor:
+        return self.table._rows.get(("result", h.shape[1]), h.shape[0],
+                                    lambda n: torch.empty(n, h.shape[1], dtype=h.dtype, device=h.device))
 
     def __call__(self, x: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
         _need_cuda(x, "x")

@@ -363,6 +363,13 @@ ATTN = [
     (MHA, [0] * 5 + [200] * 20, [1] * 25, 16, 0),
     (dict(FULL, n_heads=8, n_kv_heads=1), [20000], [2], 16, 0),
     (dict(D64, n_heads=2, n_kv_heads=1), [i * 3 for i in range(300)], [1 + i % 3 for i in range(300)], 16, 9),
+    # no more rows than requests, but all of one request's: several small units
+    (FULL, [300] + [5] * 44, [37] + [0] * 44, 16, 0),
+    (dict(SWA, keep_first=17), [700, 0] + [0] * 60, [29, 30] + [0] * 60, 32, 1),
+    (dict(G3, window=50, sinks=True), [9, 1000, 0, 0], [1, 3, 0, 0], 128, 0),
+    # few rows over many keys: parts of every size
+    (dict(FULL, n_heads=2, n_kv_heads=1), [30000, 200, 1], [1, 1, 1], 128, 0),
+    (dict(D64, n_heads=1, n_kv_heads=1, sinks=True), [40000], [300], 64, 3),
 ]
 
 
@@ -561,5 +568,65 @@ def test_paged_stack_serves_each_request_as_a_stack_of_its_own(gpu):
         feed([1, 1, 1, 1, 1], 5, replay)
     feed([1, 0, 1, 1, 0], 5, replay)
     assert stack.offset.tolist() == [191 + 6, 60 + 4, 131 + 6, 17 + 5, 1 + 5]
-    stack.table.status.item()
-    stack.caches[0].step.check()
+    # more rows than any step before: buffers grow, and the graph keeps its own
+    feed([60, 70, 1, 90, 20], 2 * T + 50)
+    feed([1, 1, 1, 1, 1], 5, replay)
+    stack.check()
+    # a step that does not fit runs without new tokens and says so
+    before = stack.offset.tolist()
+    stack(torch.zeros(5, 1024, dtype=torch.bfloat16, device=gpu), i32([600, 0, 0, 0, 0], gpu))
+    with pytest.raises(ValueError):
+        stack.check()
+    assert stack.offset.tolist() == before
+    feed([1, 1, 1, 1, 1], 5, replay)
+    stack.check()
+
+
+def test_python_refusals(gpu):
+    from mimo_moe import paged
+    from mimo_moe.layer import AttentionConfig
+    cfg = cfg_of(SWA, keep_first=4)
+    step, cache, q, kv, sinks = fill(cfg, [100, 20], [3, 1], 16, gpu, 1)
+    q = q.to(gpu)
+    plan = paged.attention_plan(step, cfg)
+    other, *_ = fill(cfg, [100, 20], [3, 1], 16, gpu, 2)
+    small = paged.PagedKVCache(cfg_of(D64), 20, 16, gpu)
+    big_pages = paged.PagedKVCache(cfg, 20, 32, gpu)
+    out = torch.empty(4, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=gpu)
+    odd = torch.empty(4 * cfg.n_heads * cfg.v_head_dim + 8, dtype=torch.bfloat16, device=gpu)[8:].view(out.shape)
+
+    def att(**kw):
+        a = dict(q=q, cache=cache, cfg=cfg, step=step, sinks=sinks, plan=plan, out=out)
+        a.update(kw)
+        return paged.attention_paged(**a)
+
+    att()
+    for kw in (dict(q=q[:3]), dict(q=q.cpu()), dict(step=other), dict(cfg=cfg_of(SWA)), dict(cfg=cfg_of(FULL)),
+               dict(cache=small), dict(cache=big_pages), dict(sinks=sinks[:5]), dict(out=out.float()),
+               dict(out=out[:, ::2]), dict(out=odd), dict(cfg=cfg_of(SWA, window=0, keep_first=4), plan=None),
+               dict(cfg=cfg_of(SWA, window=-1), plan=None)):
+        with pytest.raises(ValueError):
+            att(**kw)
+    for bad in (AttentionConfig(n_heads=6, n_kv_heads=4), AttentionConfig(n_heads=256, n_kv_heads=1),
+                cfg_of(SWA, keep_first=-1)):
+        with pytest.raises(ValueError):
+            paged.attention_plan(step, bad)
+    qkv = torch.zeros(4, cfg.qkv_width, dtype=torch.bfloat16, device=gpu)
+    for args in ((qkv[:3], cfg, cache, step), (qkv[:, 8:], cfg, cache, step), (qkv, cfg, small, step),
+                 (qkv, cfg_of(SWA, rotary_dim=33), cache, step)):
+        with pytest.raises(ValueError):
+            paged.rope_store_paged(*args)
+    table = paged.PageTable(2, 64, 8, 16, gpu)
+    for new, tokens in ((i32([1], gpu), 4), (i32([1, 1], gpu).long(), 4), (torch.ones(2, dtype=torch.int32), 4),
+                        (i32([1, 1], gpu), -1)):
+        with pytest.raises(ValueError):
+            table.step(new, tokens)
+    with pytest.raises(ValueError):
+        table.release(torch.ones(3, dtype=torch.bool, device=gpu))
+    assert table.lens.tolist() == [0, 0] and table.n_free.tolist() == [8]
+    # no rows at all
+    empty = table.step(i32([0, 0], gpu), 0)
+    c0 = paged.PagedKVCache(cfg, 8, 16, gpu)
+    assert paged.rope_store_paged(qkv[:0], cfg, c0, empty).shape[0] == 0
+    assert paged.attention_paged(q[:0], c0, cfg, empty, sinks).shape[0] == 0
+    empty.check()
