@@ -53,7 +53,8 @@ int mimo_moe_page_release(const uint8_t* done, int32_t R, int32_t* lens, int32_t
 
 /* mimo_moe_layer_rope_store with a position and a cache slot per token row: RoPE of row t's q and k heads at
  * positions[t], v * v_scale (when > 0), q to q[t], k and v to slot slots[t] of every kv head.  Rows with a negative
- * slot are left out (their q rows stay as they were); a slot outside the pool sets MIMO_ERANGE and the row's k and v
+ * slot are left out (their q rows stay as they were); the others have a slot each (two rows of one slot: either's k
+ * and v, or parts of both); a slot outside the pool sets MIMO_ERANGE and the row's k and v
  * are not stored.  rotary_dim <= 256. */
 int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
                               int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,

@@ -491,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   uint64_t* v_fixed = fix_req + 1;
   uint64_t* drain = v_fixed + 1;
   uint32_t* tslot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile uint32_t* issuer_gone = tslot + 1;  // a wait of the MMA issuer ran out
   float2* xchg = reinterpret_cast<float2*>(smem + 1024);  // [2][128] (maximum, sum) of the tiles' rows
   uint8_t* sQ = smem + kHead;
   uint8_t* sRing = sQ + 2 * S::QB;
@@ -517,6 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     mbar_init(fix_req, 1);
     mbar_init(v_fixed, 1);
     mbar_init(drain, 1);
+    *issuer_gone = 0;
     mbar_fence_init();
   }
   if (warp == 9) {
@@ -797,6 +799,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           commit(&o_full[1]);
         }
       }
+      if (!ok) *issuer_gone = 1;
       commit(drain);  // every MMA issued above has completed once this arrives
       if (!mbar_wait(drain, 0)) ok = false;
     } else if (warp == 10) {  // --------------------------------------------------- zeroes what nobody sees of V
@@ -809,7 +812,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           const int kb = g.b0 + j < bl.nkb ? g.b0 + j : bl.lb + (g.b0 + j - bl.nkb);
           const int kp = kb * 128;
           if (kp + 127 <= qlast && (kp >= bl.lo || kp + 127 < bl.keep)) continue;
-          ok = mbar_wait(fix_req, fixes++ & 1);  // the block's V is there
+          // the block's V is there.  The blocks before it may be any number, whole units among them, so this wait only
+          // ends when the issuer's own, which are for single blocks, do
+          do ok = mbar_wait(fix_req, fixes & 1);
+          while (!ok && !*issuer_gone);
+          ++fixes;
           ok = __all_sync(0xFFFFFFFFu, ok);
           if (!ok) break;
           auto zero = [&](int from, int to) {

@@ -75,8 +75,9 @@ def _page_size(page_size: int) -> int:
 
 class PageStep:
     """The row layout of one step of R requests (what page_plan writes; a program with a page allocator of its own
-    fills it itself, with a slot of its own for every row): block_table int32 [R, width], cu_q int32 [R + 1], seq_lens int32 [R] (lengths with the step's
-    tokens), positions and slots int32 [tokens].  n_free int32 [1] and status int32 [1] are page_plan's."""
+    fills it itself, with a slot of its own for every row): block_table int32 [R, width], cu_q int32 [R + 1], seq_lens
+    int32 [R] (lengths with the step's tokens), positions and slots int32 [tokens].  n_free int32 [1] and status int32
+    [1] are page_plan's."""
 
     def __init__(self, *, block_table: torch.Tensor, page_size: int, cu_q: torch.Tensor, seq_lens: torch.Tensor,
                  positions: torch.Tensor, slots: torch.Tensor, n_free: Optional[torch.Tensor] = None,
@@ -222,8 +223,8 @@ class PageTable:
         self._rows = _Rows()
 
     def step(self, new_lens: torch.Tensor, tokens: int) -> PageStep:
-        """Plan a step (page_plan) and take its lengths and free pages over.  The step's buffers are the table's: the next
-        step writes them again."""
+        """Plan a step (page_plan) and take its lengths and free pages over.  The step's buffers are the table's: the
+        next step writes them again."""
         if tokens < 0:
             raise ValueError(f"a step has no {tokens} token rows")
         R = self.requests
@@ -246,8 +247,8 @@ class PageTable:
 
 class PagedKVCache:
     """Paged KV cache of one attention layer: k [num_pages, n_kv, page_size, head_dim], v [num_pages, n_kv, page_size,
-    v_head_dim] bf16 (new and zeroed, or the tensors given).  `step` is the PageStep the layer's next call works on, `plan`
-    that step's attention plan for the layer's kind (None: made at the call)."""
+    v_head_dim] bf16 (new and zeroed, or the tensors given).  `step` is the PageStep the layer's next call works on,
+    `plan` that step's attention plan for the layer's kind (None: made at the call)."""
 
     paged = True
 
@@ -367,8 +368,10 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """mimo_moe.layer.attention for a step's token rows over the paged cache: causal; with cfg.window a sliding window,
     in which each request's first cfg.keep_first tokens stay visible; sinks float32 [n_heads].  plan: the step's
-    attention_plan for this kind of layer (made for this call when None).  Returns bf16 [tokens, n_heads, v_head_dim];
-    padding rows of a given `out` are not written, those of a new one are zero."""
+    attention_plan for this kind of layer (made for this call when None).  Cache slots that no query of the step sees
+    may hold anything; v at a position that one query sees must be finite for the request's earlier queries too.
+    Returns bf16 [tokens, n_heads, v_head_dim]; padding rows of a given `out` are not written, those of a new one are
+    zero."""
     _fits(cache, cfg, step, "attention_paged")
     T, dev = step.tokens, step.device
     q = _bf16(q, "q", (T, cfg.n_heads, cfg.head_dim), dev)
@@ -408,6 +411,7 @@ class PagedDecoderStack(DecoderStack):
             raise ValueError("empty stack")
         self.layers = list(layers)
         dev = self.layers[0].attn.w_o.device
+        self.hidden = self.layers[0].attn.w_o.shape[0]
         self.table = PageTable(max_requests, max_len, num_pages, page_size, dev)
         self.caches = [PagedKVCache(l.attn.cfg, num_pages, page_size, dev) for l in self.layers]
 
@@ -434,7 +438,12 @@ class PagedDecoderStack(DecoderStack):
 
     def __call__(self, x: torch.Tensor, new_lens: torch.Tensor) -> torch.Tensor:
         _need_cuda(x, "x")
+        if x.dim() != 2 or x.shape[1] != self.hidden or x.device != self.table.device:
+            raise ValueError(f"paged stack: x must have shape [tokens, {self.hidden}] on {self.table.device}, got "
+                             f"{tuple(x.shape)} on {x.device}")
         step = self.table.step(new_lens, x.shape[0])
+        if step.tokens == 0:
+            return x.to(torch.bfloat16)
         plans = {}
         for c in self.caches:   # one attention plan for each kind of layer
             kind = _kind(c.cfg)

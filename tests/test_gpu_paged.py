@@ -314,7 +314,9 @@ def fill(cfg, held, new, P, gpu, seed, pad=0, poison=float("nan")):
     return step, cache, q, kv, sinks
 
 
-def compare(cfg, out, q, kv, held, new, sinks, some=None):
+def compare(cfg, out, q, kv, held, new, sinks, some=None, blocks=0):
+    """blocks: of a row of more than a few thousand keys, whose float32 output is 8 accumulations a block, each off by
+    at most a unit in the last place of the row's magnitude (rounded or cut off)."""
     row = 0
     for r, (h, n) in enumerate(zip(held, new)):
         if n and (some is None or r in some):
@@ -322,7 +324,7 @@ def compare(cfg, out, q, kv, held, new, sinks, some=None):
             ref, mag = PR.attention(PR.f64(q[row:row + n]), PR.f64(K), PR.f64(V), h, cfg.scale, cfg.window,
                                     cfg.keep_first, None if sinks is None else PR.f64(sinks))
             got = PR.f64(out[row:row + n])
-            bad = ~(np.abs(got - ref) <= U * np.abs(ref) + (U + 2.0 ** -11) * mag)
+            bad = ~(np.abs(got - ref) <= U * np.abs(ref) + (U + 2.0 ** -11 + blocks * 2.0 ** -20) * mag)
             assert not bad.any(), (r, int(bad.sum()), np.argwhere(bad)[:3].tolist(), float(np.abs(got - ref).max()))
         row += n
 
@@ -580,6 +582,14 @@ def test_paged_stack_serves_each_request_as_a_stack_of_its_own(gpu):
     assert stack.offset.tolist() == before
     feed([1, 1, 1, 1, 1], 5, replay)
     stack.check()
+    # rows of another width and steps without rows leave the lengths alone
+    before = stack.offset.tolist()
+    for bad in (torch.zeros(5, 1016, device=gpu), torch.zeros(1024, device=gpu), torch.zeros(5, 1024)):
+        with pytest.raises(ValueError):
+            stack(bad, i32([1, 1, 1, 1, 1], gpu))
+    assert stack(torch.zeros(0, 1024, device=gpu), i32([0] * 5, gpu)).shape == (0, 1024)
+    stack.check()
+    assert stack.offset.tolist() == before
 
 
 def test_python_refusals(gpu):
@@ -630,3 +640,86 @@ def test_python_refusals(gpu):
     assert paged.rope_store_paged(qkv[:0], cfg, c0, empty).shape[0] == 0
     assert paged.attention_paged(q[:0], c0, cfg, empty, sinks).shape[0] == 0
     empty.check()
+
+
+def test_pages_far_into_a_pool_of_more_than_32_bits(gpu):
+    """The last pages of a pool of 2^32 values and more give the bits that the same pages of a small pool give."""
+    from mimo_moe import paged
+    cfg, P, near = cfg_of(FULL), 128, 12
+    far = 2**32 // (cfg.n_kv_heads * P * cfg.v_head_dim) + near
+    held, new = [200, 300, 0], [3, 150, 1]
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn(sum(new), cfg.qkv_width, generator=g).to(torch.bfloat16).to(gpu)
+    got = []
+    for N in (near, far):
+        table = torch.tensor([[N - 1, N - 4, -1, -1], [N - 2, N - 3, N - 5, N - 6], [N - 7, -1, -1, -1]],
+                             dtype=torch.int32, device=gpu)
+        k = torch.empty(N, cfg.n_kv_heads, P, cfg.head_dim, dtype=torch.bfloat16, device=gpu)
+        v = torch.empty(N, cfg.n_kv_heads, P, cfg.v_head_dim, dtype=torch.bfloat16, device=gpu)
+        gen = torch.Generator(gpu).manual_seed(6)
+        for t in (k, v):
+            t[N - near:].copy_(torch.randn(t[N - near:].shape, generator=gen, device=gpu))
+        cache = paged.PagedKVCache(cfg, N, P, k=k, v=v)
+        step = paged.page_plan(i32(held, gpu), i32(new, gpu), table, torch.arange(N, dtype=torch.int32, device=gpu),
+                               i32([N - 10], gpu), P, sum(new))
+        q = paged.rope_store_paged(qkv, cfg, cache, step)
+        out = paged.attention_paged(q, cache, cfg, step)
+        step.check()
+        got.append([t.cpu() for t in (q, out, k[N - near:], v[N - near:], step.slots - (N - near) * P)])
+        del cache, k, v, t
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_rows_far_into_a_step_of_more_than_32_bits(gpu):
+    """A prompt whose projection, q and output rows pass 2^31 values: its last rows."""
+    from mimo_moe import paged
+    cfg, P, n = cfg_of(SWA, sinks=False), 64, 48
+    T = 2**31 // (cfg.n_heads * cfg.v_head_dim) + 2 * n + 5
+    gen = torch.Generator(gpu).manual_seed(7)
+    qkv = torch.empty(T, cfg.qkv_width, dtype=torch.bfloat16, device=gpu)
+    for i in range(0, T, 16384):
+        qkv[i:i + 16384].copy_(torch.randn(min(16384, T - i), cfg.qkv_width, generator=gen, device=gpu))
+    table = paged.PageTable(1, T, -(-T // P), P, gpu)
+    cache = paged.PagedKVCache(cfg, table.num_pages, P, gpu)
+    step = table.step(i32([T], gpu), T)
+    q = paged.rope_store_paged(qkv, cfg, cache, step)
+    out = paged.attention_paged(q, cache, cfg, step)
+    step.check()
+    # the same rows alone: the rotation's bits, and the formula of the attention over the window they see
+    one = paged.PageStep(block_table=step.block_table, page_size=P, cu_q=i32([0, n], gpu), seq_lens=i32([T], gpu),
+                         positions=step.positions[-n:].contiguous(), slots=step.slots[-n:].contiguous())
+    k0 = cache.k.clone()
+    assert torch.equal(q[-n:], paged.rope_store_paged(qkv[-n:], cfg, cache, one))
+    assert torch.equal(k0, cache.k)
+    p = torch.arange(T - n - cfg.window, T, device=gpu)
+    page = step.block_table[0][p // P].long()
+    K, V = cache.k[page, :, p % P].cpu(), cache.v[page, :, p % P].cpu()
+    # (positions counted from the first of these keys: the rows see the same of them)
+    compare(cfg, out[-n:], q[-n:].cpu(), [(K, V)], [cfg.window], [n], None)
+
+
+def test_attention_paged_in_a_call_of_seconds(gpu):
+    """Waits are bounded, and none of them is for a whole call: a prompt of whole blocks, one page for all of them, and
+    behind it a request whose last block is ragged."""
+    from mimo_moe import paged
+    cfg, P, T = cfg_of(dict(D64, n_heads=1, n_kv_heads=1)), 128, 3 * 2**20
+    gen = torch.Generator(gpu).manual_seed(8)
+    cache = paged.PagedKVCache(cfg, 2, P, gpu)
+    cache.k.copy_(torch.randn(cache.k.shape, generator=gen, device=gpu))
+    cache.v.copy_(torch.randn(cache.v.shape, generator=gen, device=gpu))
+    small = 100
+    table = torch.zeros(2, T // P, dtype=torch.int32, device=gpu)
+    table[1] = 1
+    q = torch.randn(T + small, 1, cfg.head_dim, generator=gen, device=gpu).to(torch.bfloat16)
+    rows = torch.zeros(T + small, dtype=torch.int32, device=gpu)
+    step = paged.PageStep(block_table=table, page_size=P, cu_q=i32([0, T, T + small], gpu),
+                          seq_lens=i32([T, small], gpu), positions=rows, slots=rows)
+    out = paged.attention_paged(q, cache, cfg, step)
+    step.check()
+    K, V = cache.k[1].transpose(0, 1)[:small].cpu(), cache.v[1].transpose(0, 1)[:small].cpu()
+    compare(cfg, out[T:], q[T:].cpu(), [(K, V)], [0], [small], None)
+    # a row that ends with the k-th repetition of the page sees every key k times: the softmax of the page alone
+    K, V = cache.k[0].transpose(0, 1).cpu(), cache.v[0].transpose(0, 1).cpu()
+    for k in (1, 1000, T // P):
+        compare(cfg, out[k * P - 1:k * P], q[k * P - 1:k * P].cpu(), [(K, V)], [P - 1], [1], None, blocks=k)
