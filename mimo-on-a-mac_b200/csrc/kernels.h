@@ -341,7 +341,6 @@ struct PagedRopeParams {
   uint16_t *q, *k, *v;               // q [T][nq][dqk], pools [num_pages][nkv][page][d]
   int32_t* status;
   int T, nq, nkv, dqk, dv, rot, num_pages, page_shift, has_vscale;
-  int rows;         // token rows of a CTA
   float v_scale;    // already a bf16 value
   double log_base;  // ln(rope_theta)
 };
@@ -375,7 +374,7 @@ size_t paged_attn_part_rows(int T, int R, int G, int num_sms);  // rows of parts
 cudaError_t launch_attn_plan(AttnPlanParams& p, cudaStream_t st);
 cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st);
 cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st);
-cudaError_t launch_paged_rope(PagedRopeParams& p, cudaStream_t st);
+cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st);
 cudaError_t launch_paged_attention(PagedAttnParams& p, int num_sms, cudaStream_t st);
 
 }  // namespace mimo

@@ -180,18 +180,14 @@ __global__ void __launch_bounds__(kPlanThreads) page_release_kernel(PageReleaseP
   if (tid == 0) *p.n_free = nfree + n;
 }
 
-// RoPE + append.  A CTA takes a few token rows (and, when there are few, a share of each row's work): the cosines and
-// sines of their rotary pairs into shared memory, then the rows in pieces of 16 bytes, a rotary piece together with the
-// one half the rotary dims away.  Every value is read once and written once: 2048 rows of 64 + 4 heads of 192 are 111 MB
-// and take 32 us (3.5 TB/s), 16000 of 64 + 8 heads 198 us (4.4 TB/s); what is left is the loads in flight that four CTAs
-// of 64 registers a thread hold on an SM (more threads of fewer registers, or fewer pieces each, were slower).
+// RoPE + append.  Every value is read once and written once, so memory is what bounds it: a row goes through shared memory
+// in bulk copies where it fits there (paged_rope_rows_kernel), else through registers (paged_rope_kernel).
 //
 // The angle pos * theta^(-2i/rot), its reduction to [-pi, pi], sine and cosine are float64.  The rotation is float32, with
 // the cosine (and sine) as a sum of its first 16 bits, whose product with a bf16 value is exact, and the rest: then even
 // x1 cos - x2 sin that almost cancels is off by no more than 2^-24 of itself and 2^-40 (|x1| + |x2|), and has the bits of
 // the one-sequence kernel's float64 rotation on all but one value in 10^5, without converting every value to float64.
 constexpr int kRopeThreads = 256;
-constexpr int kRopeRows = 4;
 
 // Two float32 values rounded to nearest-even bf16 in one conversion: lo in bits 0-15, hi in bits 16-31.
 __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
@@ -205,11 +201,20 @@ __device__ __forceinline__ float cos_part(float x1, float x2, float4 t) {  // x1
 __device__ __forceinline__ float sin_part(float x1, float x2, float4 t) {  // x1 sin + x2 cos
   return fmaf(x1, t.y, x2 * t.x) + fmaf(x1, t.w, x2 * t.z);
 }
+// The cosine and sine of an angle: first parts, rests.
+__device__ __forceinline__ float4 rotary(double a) {
+  const double turns = rint(a * 0.15915494309189535);                                         // 1 / 2 pi
+  const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, a));  // 2 pi in two parts
+  double sn, cn;
+  sincos(r, &sn, &cn);
+  const float c0 = __uint_as_float(__float_as_uint((float)cn) & 0xFFFFFF00u);
+  const float s0 = __uint_as_float(__float_as_uint((float)sn) & 0xFFFFFF00u);
+  return make_float4(c0, s0, (float)(cn - (double)c0), (float)(sn - (double)s0));
+}
 // Two rotary pairs: x1 and x2 become the rotated values.
-__device__ __forceinline__ void rotate2(uint32_t& x1, uint32_t& x2, const float4* t) {
+__device__ __forceinline__ void rotate2(uint32_t& x1, uint32_t& x2, float4 ta, float4 tb) {
   const float a1 = bf16_to_f32(x1 & 0xFFFFu), a2 = bf16_to_f32(x2 & 0xFFFFu);
   const float b1 = bf16_to_f32(x1 >> 16), b2 = bf16_to_f32(x2 >> 16);
-  const float4 ta = t[0], tb = t[1];
   x1 = pack_bf16x2(cos_part(a1, a2, ta), cos_part(b1, b2, tb));
   x2 = pack_bf16x2(sin_part(a1, a2, ta), sin_part(b1, b2, tb));
 }
@@ -217,114 +222,143 @@ __device__ __forceinline__ uint32_t scaled(uint32_t w, float s) {
   return pack_bf16x2(bf16_to_f32(w & 0xFFFFu) * s, bf16_to_f32(w >> 16) * s);
 }
 
-// VEC: the rotary dims are a multiple of 16, so that a row is whole 16-byte pieces; otherwise value by value.
-template <bool VEC>
-__global__ void __launch_bounds__(kRopeThreads, 4) paged_rope_kernel(PagedRopeParams p) {
-  __shared__ float4 cs[kRopeRows * 128];
+// Whole token rows through shared memory, in CTAs that each hold one: a row of projections comes in with one bulk copy,
+// its rotary pairs and values are rotated and scaled in place while other CTAs' rows are on their way, and it goes out
+// with one bulk copy for q (the row's q heads lie as they do in the input) and one for each kv head's k and v.  What is in
+// flight costs no registers: six rows of 27 KB an SM.  2048 rows of 64 + 4 heads of 192 are 111 MB and take 22.8 us (4.9
+// TB/s; 32 through registers), 16000 of them 154 us (5.6 TB/s; 198), 8 rows 2.6 us (2.7).
+constexpr size_t kRowSmem = 232448;  // a CTA's most
+constexpr int kRowHead = 128 * 16 + 128 * 8 + 128;  // cosines and sines, frequencies, the barrier
+
+__device__ __forceinline__ void bulk_s2g(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n" ::"l"(dst), "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_rope_rows_kernel(PagedRopeParams p) {
+  extern __shared__ __align__(128) uint8_t rows_smem[];
+  float4* cs = reinterpret_cast<float4*>(rows_smem);  // [8][rot / 16]: pair 8 k + e of a head at e * (rot / 16) + k
+  double* freq = reinterpret_cast<double*>(rows_smem + 128 * 16);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(rows_smem + 128 * 24);
+  uint8_t* row = rows_smem + kRowHead;
+  const int half = p.rot / 2, rp = p.rot / 16, tid = threadIdx.x;
+  const int heads = p.nq + p.nkv, page_mask = (1 << p.page_shift) - 1;
+  const uint32_t qk_bytes = (uint32_t)heads * p.dqk * 2, bytes = qk_bytes + (uint32_t)p.nkv * p.dv * 2;
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    mbar_fence_init();
+  }
+  if (tid < half) freq[tid] = exp(-(double)(2 * tid) / (double)p.rot * p.log_base);
+  __syncthreads();
+  pdl_wait();  // the projection rows and the plan come from preceding kernels (programmatic dependent launch)
+  pdl_launch_dependents();
+  uint32_t phase = 0;
+  int t = blockIdx.x, slot = -1, pos = 0;
+  if (t < p.T) slot = p.slots[t], pos = p.positions[t];
+  for (; t < p.T; t += gridDim.x) {
+    const int my_slot = slot, my_pos = pos;
+    if (t + (int)gridDim.x < p.T) slot = p.slots[t + gridDim.x], pos = p.positions[t + gridDim.x];
+    if (my_slot < 0) continue;
+    if (tid < 32) {
+      asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // the row before has left
+      __syncwarp();
+      if (tid == 0) {
+        mbar_arrive_expect_tx(bar, bytes);
+        bulk_g2s(row, reinterpret_cast<const uint8_t*>(p.qkv) + (size_t)t * bytes, bytes, bar, l2_evict_first_policy());
+      }
+    }
+    if (tid < half) {
+      const double a = (double)my_pos * freq[tid];
+      cs[(tid & 7) * rp + (tid >> 3)] = rotary(a);
+    }
+    const bool ok = __syncthreads_and(mbar_wait(bar, phase));
+    phase ^= 1;
+    if (!ok) {
+      if (tid == 0) set_status(p.status, MIMO_ETIMEOUT);
+      break;
+    }
+    for (int i = tid; i < heads * rp; i += THREADS) {
+      const int hd = i / rp, k = i - hd * rp;
+      uint4* a4 = reinterpret_cast<uint4*>(row + (uint32_t)hd * p.dqk * 2) + k;
+      // heads may lie a multiple of all banks apart: every other one is read from its second piece on
+      uint4 *f = a4 + (hd & 1 ? rp : 0), *g = a4 + (hd & 1 ? 0 : rp);
+      const uint4 u = *f, w = *g;
+      uint4 x = hd & 1 ? w : u, z = hd & 1 ? u : w;
+      const float4* e = cs + k;
+      rotate2(x.x, z.x, e[0], e[rp]), rotate2(x.y, z.y, e[2 * rp], e[3 * rp]);
+      rotate2(x.z, z.z, e[4 * rp], e[5 * rp]), rotate2(x.w, z.w, e[6 * rp], e[7 * rp]);
+      *f = hd & 1 ? z : x;
+      *g = hd & 1 ? x : z;
+    }
+    if (p.has_vscale)
+      for (int i = tid; i < p.nkv * p.dv / 8; i += THREADS) {
+        uint4* w = reinterpret_cast<uint4*>(row + qk_bytes) + i;
+        *w = make_uint4(scaled(w->x, p.v_scale), scaled(w->y, p.v_scale), scaled(w->z, p.v_scale),
+                        scaled(w->w, p.v_scale));
+      }
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    __syncthreads();
+    if (tid < 32) {
+      const int page = my_slot >> p.page_shift, at = my_slot & page_mask;
+      const bool store = page < p.num_pages;
+      if (tid == 0) {
+        if (!store) set_status(p.status, MIMO_ERANGE);
+        bulk_s2g(p.q + (size_t)t * p.nq * p.dqk, row, (uint32_t)p.nq * p.dqk * 2);
+      }
+      if (store)
+        for (int h = tid; h < p.nkv; h += 32) {
+          const size_t to = (((size_t)page * p.nkv + h) << p.page_shift) + at;
+          bulk_s2g(p.k + to * p.dqk, row + (uint32_t)(p.nq + h) * p.dqk * 2, (uint32_t)p.dqk * 2);
+          bulk_s2g(p.v + to * p.dv, row + qk_bytes + (uint32_t)h * p.dv * 2, (uint32_t)p.dv * 2);
+        }
+      asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
+    }
+  }
+  if (tid < 32) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
+}
+
+// What the other does not take: rotary dims that are no multiple of 16, and rows wider than shared memory.  A CTA takes a
+// share of one row, value by value.
+__global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(PagedRopeParams p) {
+  __shared__ float4 cs[128];
   __shared__ double freq[128];
-  const int half = p.rot / 2, tid = threadIdx.x;
-  const int t0 = blockIdx.x * p.rows, nt = min(p.rows, p.T - t0);
+  const int half = p.rot / 2, tid = threadIdx.x, t = blockIdx.x;
   // the frequencies need no input: before the wait for the kernels before this one
   if (tid < half) freq[tid] = exp(-(double)(2 * tid) / (double)p.rot * p.log_base);
   __syncthreads();
   pdl_wait();  // the projection rows and the plan come from preceding kernels (programmatic dependent launch)
   pdl_launch_dependents();
-  for (int i = tid; i < nt * half; i += kRopeThreads) {
-    const double a = (double)p.positions[t0 + i / half] * freq[i % half];
-    const double turns = rint(a * 0.15915494309189535);                                             // 1 / 2 pi
-    const double r = fma(-turns, 2.4492935982947064e-16, fma(-turns, 6.283185307179586, a));  // 2 pi in two parts
-    double sn, cn;
-    sincos(r, &sn, &cn);
-    const float c0 = __uint_as_float(__float_as_uint((float)cn) & 0xFFFFFF00u);
-    const float s0 = __uint_as_float(__float_as_uint((float)sn) & 0xFFFFFF00u);
-    cs[i] = make_float4(c0, s0, (float)(cn - (double)c0), (float)(sn - (double)s0));
-  }
+  const int slot = p.slots[t];
+  if (slot < 0) return;
+  if (tid < half) cs[tid] = rotary((double)p.positions[t] * freq[tid]);
   __syncthreads();
-  const int heads = p.nq + p.nkv, page_mask = (1 << p.page_shift) - 1;
-  const size_t rowlen = (size_t)heads * p.dqk + (size_t)p.nkv * p.dv;
-  // pieces of a row: the heads' rotary pairs of pieces, their other pieces, the value rows': one after the other, so that
-  // a warp has one kind to do (with each head's together, every warp ran the rotation for a fifth of its lanes)
-  const int rp = VEC ? p.rot / 16 : half, hp = (p.dqk - p.rot) / (VEC ? 8 : 1), vp = p.dv / (VEC ? 8 : 1);
-  const int per_row = heads * (rp + hp) + p.nkv * vp;
-  const int share = (per_row + gridDim.y - 1) / gridDim.y;
-  const int first = blockIdx.y * share, last = min(per_row, first + share);
-  for (int tt = 0; tt < nt; ++tt) {
-    const int t = t0 + tt, slot = p.slots[t];
-    if (slot < 0) continue;
-    const int page = slot >> p.page_shift, at = slot & page_mask;
-    const bool store = page < p.num_pages;
-    if (!store && tid == 0) set_status(p.status, MIMO_ERANGE);
-    const uint16_t* row = p.qkv + (size_t)t * rowlen;
-    const float4* c = cs + tt * half;
-    // where the head or value row of piece i comes from and goes to (null: nowhere), which piece of it it is (a rotary
-    // pair's first), and its kind
-    enum { kRotary, kCopy, kValue };
-    auto piece = [&](int i, const uint16_t*& src, uint16_t*& dst, int& k) -> int {
-      int kind = kRotary, n = rp;
-      if (i >= heads * rp) i -= heads * rp, kind = kCopy, n = hp;
-      if (kind == kCopy && i >= heads * hp) i -= heads * hp, kind = kValue, n = vp;
-      const int hd = i / n;
-      k = i - hd * n;
-      if (kind == kValue) {
-        src = row + (size_t)heads * p.dqk + (size_t)hd * p.dv;
-        dst = store ? p.v + ((((size_t)page * p.nkv + hd) << p.page_shift) + at) * p.dv : nullptr;
+  const int page = slot >> p.page_shift, at = slot & ((1 << p.page_shift) - 1);
+  const bool store = page < p.num_pages;
+  if (!store && tid == 0) set_status(p.status, MIMO_ERANGE);
+  const int heads = p.nq + p.nkv, qk = heads * (p.dqk - half), all = qk + p.nkv * p.dv;  // a rotary pair counts once
+  const uint16_t* row = p.qkv + (size_t)t * ((size_t)heads * p.dqk + (size_t)p.nkv * p.dv);
+  const int share = (all + gridDim.y - 1) / gridDim.y, last = min(all, (int)(blockIdx.y + 1) * share);
+  for (int i = blockIdx.y * share + tid; i < last; i += kRopeThreads) {
+    if (i < qk) {
+      const int hd = i / (p.dqk - half), e = i - hd * (p.dqk - half);  // pairs 0 .. half - 1, then the other dims
+      const uint16_t* src = row + (size_t)hd * p.dqk;
+      uint16_t* dst = hd < p.nq ? p.q + ((size_t)t * p.nq + hd) * p.dqk
+                      : store   ? p.k + ((((size_t)page * p.nkv + (hd - p.nq)) << p.page_shift) + at) * p.dqk
+                                : nullptr;
+      if (dst == nullptr) continue;
+      if (e < half) {
+        const float x1 = bf16_to_f32(src[e]), x2 = bf16_to_f32(src[e + half]);
+        dst[e] = (uint16_t)f32_to_bf16(cos_part(x1, x2, cs[e]));
+        dst[e + half] = (uint16_t)f32_to_bf16(sin_part(x1, x2, cs[e]));
       } else {
-        if (kind == kCopy) k += 2 * rp;
-        src = row + (size_t)hd * p.dqk;
-        dst = hd < p.nq ? p.q + ((size_t)t * p.nq + hd) * p.dqk
-              : store   ? p.k + ((((size_t)page * p.nkv + (hd - p.nq)) << p.page_shift) + at) * p.dqk
-                        : nullptr;
+        dst[e + half] = src[e + half];
       }
-      return kind;
-    };
-    if constexpr (VEC) {
-      constexpr int U = 4;  // pieces in flight a thread
-      for (int i0 = first + tid; i0 < last; i0 += U * kRopeThreads) {
-        uint4 a[U], b[U];
-        uint16_t* dst[U];
-        int k[U], kind[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int i = i0 + u * kRopeThreads;
-          const uint16_t* src;
-          dst[u] = nullptr;
-          if (i < last) kind[u] = piece(i, src, dst[u], k[u]);
-          if (dst[u] == nullptr) continue;
-          a[u] = __ldg(reinterpret_cast<const uint4*>(src) + k[u]);
-          if (kind[u] == kRotary) b[u] = __ldg(reinterpret_cast<const uint4*>(src) + k[u] + rp);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (dst[u] == nullptr) continue;
-          uint4* d4 = reinterpret_cast<uint4*>(dst[u]) + k[u];
-          uint4 w = a[u];
-          if (kind[u] == kRotary) {
-            uint4 z = b[u];
-            const float4* e = c + k[u] * 8;
-            rotate2(w.x, z.x, e), rotate2(w.y, z.y, e + 2), rotate2(w.z, z.z, e + 4), rotate2(w.w, z.w, e + 6);
-            d4[rp] = z;
-          } else if (kind[u] == kValue && p.has_vscale) {
-            w = make_uint4(scaled(w.x, p.v_scale), scaled(w.y, p.v_scale), scaled(w.z, p.v_scale),
-                           scaled(w.w, p.v_scale));
-          }
-          *d4 = w;
-        }
-      }
-    } else {
-      for (int i = first + tid; i < last; i += kRopeThreads) {
-        const uint16_t* src;
-        uint16_t* dst;
-        int k;
-        const int kind = piece(i, src, dst, k);
-        if (dst == nullptr) continue;
-        if (kind == kRotary) {
-          const float x1 = bf16_to_f32(src[k]), x2 = bf16_to_f32(src[k + half]);
-          dst[k] = (uint16_t)f32_to_bf16(cos_part(x1, x2, c[k]));
-          dst[k + half] = (uint16_t)f32_to_bf16(sin_part(x1, x2, c[k]));
-        } else {
-          dst[k] = kind == kValue && p.has_vscale ? (uint16_t)f32_to_bf16(bf16_to_f32(src[k]) * p.v_scale) : src[k];
-        }
-      }
+    } else if (store) {
+      const int hd = (i - qk) / p.dv, e = i - qk - hd * p.dv;
+      const uint16_t x = row[(size_t)heads * p.dqk + (size_t)hd * p.dv + e];
+      p.v[((((size_t)page * p.nkv + hd) << p.page_shift) + at) * p.dv + e] =
+          p.has_vscale ? (uint16_t)f32_to_bf16(bf16_to_f32(x) * p.v_scale) : x;
     }
   }
 }
@@ -341,17 +375,36 @@ cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st) {
   return launch_k(page_release_kernel, dim3(1), dim3(kPlanThreads), (size_t)(p.R + 1) * 4, st, p);
 }
 
-cudaError_t launch_paged_rope(PagedRopeParams& p, cudaStream_t st) {
-  const bool vec = p.rot % 16 == 0;
-  const int per_row = (p.nq + p.nkv) * (vec ? (p.dqk - p.rot / 2) / 8 : p.dqk - p.rot / 2) +
-                      p.nkv * (vec ? p.dv / 8 : p.dv);
-  // four rows a CTA once that gives every SM one (2048 rows: 32.1 us against 33.5 with one row a CTA, 16000: 198 against
-  // 217), else one, and a share of it: down to one piece a thread (8 rows: 3.0 us)
-  p.rows = p.T >= kRopeRows * 148 ? kRopeRows : 1;
-  const int ctas = (p.T + p.rows - 1) / p.rows, most = (per_row + kRopeThreads - 1) / kRopeThreads;
-  const int shares = std::max(1, std::min(most, 4 * 148 / ctas));
-  return launch_k(vec ? paged_rope_kernel<true> : paged_rope_kernel<false>, dim3(ctas, shares), dim3(kRopeThreads), 0,
-                  st, p);
+namespace {
+template <int THREADS>
+cudaError_t launch_rope_rows(const PagedRopeParams& p, size_t smem, int fit, cudaStream_t st) {
+  static bool attr_set[128] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 128 && !attr_set[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(paged_rope_rows_kernel<THREADS>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRowSmem);
+    if (e != cudaSuccess) return e;
+    attr_set[dev] = true;
+  }
+  const int most = 148 * fit, rounds = (p.T + most - 1) / most;  // all CTAs have the same number of rows, or one less
+  return launch_k(paged_rope_rows_kernel<THREADS>, dim3((p.T + rounds - 1) / rounds), dim3(THREADS), smem, st, p);
+}
+}  // namespace
+
+cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st) {
+  const size_t smem = kRowHead + ((size_t)(p.nq + p.nkv) * p.dqk + (size_t)p.nkv * p.dv) * 2;
+  if (p.rot % 16 == 0 && smem <= kRowSmem) {
+    const int fit = (int)std::min<size_t>(16, (228 * 1024) / (smem + 1024));  // CTAs an SM
+    // A CTA of 128 threads keeps up with memory where several rows of an SM are worked on at once; alone, 384 threads are
+    // through its row sooner (8 rows of 64 + 4 heads: 2.6 us against 2.9; 16000 of 32 + 8 heads of 128 with 256 threads:
+    // 105 us against 79, as fewer CTAs fit).
+    return p.T <= 148 || fit < 3 ? launch_rope_rows<384>(p, smem, fit, st) : launch_rope_rows<128>(p, smem, fit, st);
+  }
+  // shares of a row down to a value a thread while there are fewer rows than four for each SM
+  const int all = (p.nq + p.nkv) * (p.dqk - p.rot / 2) + p.nkv * p.dv;
+  const int shares = std::max(1, std::min((all + kRopeThreads - 1) / kRopeThreads, 4 * 148 / p.T));
+  return launch_k(paged_rope_kernel, dim3(p.T, shares), dim3(kRopeThreads), 0, st, p);
 }
 
 }  // namespace mimo

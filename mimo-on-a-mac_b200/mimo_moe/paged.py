@@ -33,7 +33,7 @@ _HERE = contextlib.nullcontext()
 
 def _on(dev: torch.device):
     """The context in which kernels launch on `dev` (nothing to do when it is the current device)."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
 def _stream(dev: torch.device) -> int:
@@ -41,8 +41,8 @@ def _stream(dev: torch.device) -> int:
 
 
 def _int32(t: torch.Tensor, name: str, shape, dev=None) -> torch.Tensor:
-    if t.dtype is torch.int32 and t.is_cuda and t.shape == shape and t.is_contiguous() and (dev is None
-                                                                                          or t.device == dev):
+    if t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() and (t.is_cuda if dev is None
+                                                                              else t.device == dev):
         return t
     _need_cuda(t, name)
     if dev is not None and t.device != dev:

@@ -209,6 +209,12 @@ ROPES = [
     (dict(FULL, rotary_dim=0), [5], [4], 64, 0, None),
     (dict(n_heads=3, n_kv_heads=1, head_dim=40, v_head_dim=24, rotary_dim=8), [0, 4], [50, 1], 16, 5, 0.707),
     (MHA, [40], [2500], 16, 0, None),
+    (FULL, [3, 0], [900, 500], 64, 300, 0.707),                           # several rows a CTA, the last ones padding
+    (dict(FULL, n_heads=200), [0], [200], 16, 200, 0.5),                  # rows of 80 KB
+    (dict(FULL, n_heads=560, n_kv_heads=2), [11], [150], 16, 1, 0.5),     # of 217 KB
+    (dict(FULL, n_heads=600, n_kv_heads=4), [1], [150], 16, 1, 0.5),      # wider than shared memory
+    (dict(D128, n_heads=1, n_kv_heads=1), [0], [5000], 128, 7, 0.5),
+    (dict(n_heads=2, n_kv_heads=2, head_dim=256, v_head_dim=8, rotary_dim=256), [100], [300], 16, 1, None),
 ]
 
 
