@@ -375,6 +375,10 @@ ATTN = [
     (FULL, [300] + [5] * 44, [37] + [0] * 44, 16, 0),
     (dict(SWA, keep_first=17), [700, 0] + [0] * 60, [29, 30] + [0] * 60, 32, 1),
     (dict(G3, window=50, sinks=True), [9, 1000, 0, 0], [1, 3, 0, 0], 128, 0),
+    # windows of more blocks than a unit that is never cut has, and of as many
+    (dict(SWA, window=1000, keep_first=200), [5000, 3000, 0], [1, 1, 700], 16, 0),
+    (dict(G3, window=700), [4000, 300], [40, 1], 64, 2),
+    (dict(D64, n_heads=1, n_kv_heads=1, window=257, keep_first=3, sinks=True), [4000, 90], [1, 1], 64, 0),
     # few rows over many keys: parts of every size
     (dict(FULL, n_heads=2, n_kv_heads=1), [30000, 200, 1], [1, 1, 1], 128, 0),
     (dict(D64, n_heads=1, n_kv_heads=1, sinks=True), [40000], [300], 64, 3),
