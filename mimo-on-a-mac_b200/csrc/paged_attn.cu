@@ -24,12 +24,13 @@
 //   warp 10          zeroes the V rows that no query of the unit sees: such slots may hold anything, and 0 * NaN is not 0.
 // Every wait is bounded and sets MIMO_ETIMEOUT; the producers drain their copies and the issuer its MMAs before exit.
 //
-// What bounds it (B200, 64 heads of 192 / 128 over 4 kv heads): a prompt's chunk of 4096 tokens on 12288 takes 3.15 M cycles
-// an SM, 64% of them with the tensor core at work (1.33 PFLOP/s alone, 1.1 under the power cap): a tile's round of softmax
-// (2000 cycles), P V and S (1420) and four hand-overs is 4100 cycles, in which the tensor core works 2 x 1280.  Without
-// any exponential it is still 3770; two threads a row, two issuing warps, P in halves and a helper for the issuer's waits
-// were all slower.  64 decoding requests (580 MB of K and V) take 111 us, 5.2 TB/s; 8 of them at 4096 tokens (84 MB) 25 us,
-// of which 9 pass before the first product: the plan, the table, K and V come from HBM one after the other.
+// What bounds it (B200, 64 heads of 192 / 128 over 4 kv heads): a prompt's chunk of 4096 tokens on 12288 takes 3.5 M
+// cycles an SM, 58% of them with the tensor core at work, and 2.1 ms under the power cap (1.14 PFLOP/s; a form of 3.15 M
+// cycles and more instructions took as long).  A tile's round of softmax (2000 cycles), P V and S (1420) and four
+// hand-overs is 4100 cycles and more, in which the tensor core works 2 x 1280.  Without any exponential it is still 3770;
+// two threads a row, two issuing warps, P in halves and a helper for the issuer's waits were all slower.  64 decoding
+// requests (580 MB of K and V) take 111 us, 5.2 TB/s; 8 of them at 4096 tokens (84 MB) 25 us, of which 9 pass before the
+// first product: the plan, the table, K and V come from HBM one after the other.
 #include <cstring>
 #include <type_traits>
 

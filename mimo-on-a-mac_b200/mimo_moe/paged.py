@@ -240,6 +240,10 @@ class PageTable:
         self._state.copy_(self._after)
         return out
 
+    def last_rows(self) -> torch.Tensor:
+        """PageStep.last_rows of the step planned last."""
+        return self._cu_q[1:] - 1
+
     def release(self, done: torch.Tensor) -> None:
         """Give back the pages of the requests with done[r]."""
         page_release(done, self.lens, self.block_table, self.free_pages, self.n_free, self.page_size, self.status)

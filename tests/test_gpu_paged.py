@@ -580,6 +580,7 @@ def test_paged_stack_serves_each_request_as_a_stack_of_its_own(gpu):
         feed([1, 1, 1, 1, 1], 5, replay)
     feed([1, 0, 1, 1, 0], 5, replay)
     assert stack.offset.tolist() == [191 + 6, 60 + 4, 131 + 6, 17 + 5, 1 + 5]
+    assert stack.table.last_rows().tolist() == [0, 0, 1, 2, 2]   # of the step [1, 0, 1, 1, 0]
     # more rows than any step before: buffers grow, and the graph keeps its own
     feed([60, 70, 1, 90, 20], 2 * T + 50)
     feed([1, 1, 1, 1, 1], 5, replay)
