@@ -13,7 +13,7 @@
  * cache slot is page * page_size + position % page_size.  All layers share one table: a page number names the same
  * positions in every layer's pool.
  *
- * Every pointer is a device pointer, 16-byte aligned where it holds bf16 values.  Errors that the kernels find in
+ * A step has at most 2^30 token rows.  Every pointer is a device pointer, 16-byte aligned where it holds bf16 values.  Errors that the kernels find in
  * device data (MIMO_ERANGE: no free page left, a length outside the table, a page outside the pool) go to the
  * optional status word; no device value makes a kernel read or write outside the arrays it is given.
  */

@@ -1143,6 +1143,7 @@ int mimo_moe_layer_add(const uint16_t* a, const uint16_t* b, int64_t n, uint16_t
 // ------------------------------------------------------------------ paged serving (include/mimo_moe_paged.h)
 namespace {
 constexpr int kMaxRequests = 4096;
+constexpr int kMaxTokens = 1 << 30;  // row numbers and a grid's stride beyond them are int32; a row's values too
 int page_shift_of(int32_t page_size) {  // log2 of a supported page size, else -1
   for (int s = 4; s <= 7; ++s)
     if (page_size == 1 << s) return s;
@@ -1161,7 +1162,7 @@ int mimo_moe_page_plan(const int32_t* lens, const int32_t* new_lens, int32_t R, 
                        int32_t page_size, int32_t tokens, int32_t* cu_q, int32_t* seq_lens, int32_t* n_free_out,
                        int32_t* positions, int32_t* slots, int32_t* status, void* stream) {
   if (!lens || !new_lens || !block_table || !free_pages || !n_free || !cu_q || !seq_lens || !n_free_out ||
-      (tokens > 0 && (!positions || !slots)) || tokens < 0 || bad_pool(num_pages, page_size) ||
+      (tokens > 0 && (!positions || !slots)) || tokens < 0 || tokens > kMaxTokens || bad_pool(num_pages, page_size) ||
       bad_table(R, table_width, page_size) || seq_lens == lens || seq_lens == new_lens || n_free_out == n_free)
     return MIMO_EINVAL;
   PagePlanParams p{};
@@ -1191,9 +1192,10 @@ int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_hea
                               float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
                               int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages, int32_t* status,
                               void* stream) {
-  if (!qkv || !positions || !slots || !q || !k_pages || !v_pages || tokens < 1 || n_heads < 1 || n_kv_heads < 1 ||
-      head_dim < 8 || v_head_dim < 8 || head_dim % 8 || v_head_dim % 8 || rotary_dim < 0 || rotary_dim % 2 ||
-      rotary_dim > head_dim || rotary_dim > 256 || !(rope_theta > 0.f) || !(v_scale >= 0.f) ||
+  if (!qkv || !positions || !slots || !q || !k_pages || !v_pages || tokens < 1 || tokens > kMaxTokens || n_heads < 1 ||
+      n_kv_heads < 1 || head_dim < 8 || v_head_dim < 8 || head_dim % 8 || v_head_dim % 8 || rotary_dim < 0 || rotary_dim % 2 ||
+      rotary_dim > head_dim || rotary_dim > 256 ||
+      ((int64_t)n_heads + n_kv_heads) * head_dim + (int64_t)n_kv_heads * v_head_dim > kMaxTokens || !(rope_theta > 0.f) || !(v_scale >= 0.f) ||
       bad_pool(num_pages, page_size) || !a16(qkv) || !a16(q) || !a16(k_pages) || !a16(v_pages))
     return MIMO_EINVAL;
   PagedRopeParams p{};
@@ -1220,7 +1222,7 @@ int32_t attn_plan_key(int32_t T, int32_t R, int32_t n_heads, int32_t n_kv_heads,
 }  // namespace
 
 size_t mimo_moe_paged_attention_plan_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads) {
-  if (tokens < 1 || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads)) return 0;
+  if (tokens < 1 || tokens > kMaxTokens || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads)) return 0;
   return attn_plan_bytes(tokens, R, n_heads / n_kv_heads, n_kv_heads, num_sms_current());
 }
 
@@ -1228,7 +1230,7 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
                                   int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,
                                   int32_t table_width, int32_t page_size, void* plan, size_t plan_bytes,
                                   int32_t* status, void* stream) {
-  if (!cu_q || !seq_lens || !plan || tokens < 1 || bad_heads(n_heads, n_kv_heads) || window < 0 || keep_first < 0 ||
+  if (!cu_q || !seq_lens || !plan || tokens < 1 || tokens > kMaxTokens || bad_heads(n_heads, n_kv_heads) || window < 0 || keep_first < 0 ||
       (keep_first > 0 && window == 0) || page_shift_of(page_size) < 0 || bad_table(R, table_width, page_size) ||
       !a16(plan) || plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads))
     return MIMO_EINVAL;
@@ -1244,7 +1246,9 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
 
 size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads,
                                                 int32_t v_head_dim) {
-  if (tokens < 1 || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads) || v_head_dim < 1) return 0;
+  if (tokens < 1 || tokens > kMaxTokens || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads) ||
+      v_head_dim < 1)
+    return 0;
   return paged_attn_part_rows(tokens, R, n_heads / n_kv_heads, num_sms_current()) * ((size_t)v_head_dim + 2) * 4;
 }
 
@@ -1255,7 +1259,7 @@ int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const u
                              const void* plan, size_t plan_bytes, uint16_t* out, void* workspace,
                              size_t workspace_bytes, int32_t* status, void* stream) {
   if (!q || !k_pages || !v_pages || !block_table || !plan || !out || !workspace || tokens < 1 ||
-      bad_heads(n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
+      tokens > kMaxTokens || bad_heads(n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
       keep_first < 0 || (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) ||
       (int64_t)num_pages * n_kv_heads >= INT32_MAX || bad_table(R, table_width, page_size) || !a16(q) ||
       !a16(k_pages) || !a16(v_pages) || !a32(out) || !a16(plan) || !a32(workspace) ||

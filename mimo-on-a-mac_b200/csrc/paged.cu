@@ -277,6 +277,7 @@ __global__ void __launch_bounds__(THREADS) paged_rope_rows_kernel(PagedRopeParam
     phase ^= 1;
     if (!ok) {
       if (tid == 0) set_status(p.status, MIMO_ETIMEOUT);
+      mbar_wait(bar, phase ^ 1);  // the copy may still be landing
       break;
     }
     for (int i = tid; i < heads * rp; i += THREADS) {

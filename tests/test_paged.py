@@ -33,7 +33,7 @@ def plan_args(**kw):
                                  dict(cu=None), dict(seq=None), dict(n_out=None), dict(pos=None), dict(slots=None),
                                  dict(R=0), dict(R=4097), dict(width=0), dict(pages=0), dict(P=0), dict(P=8), dict(P=48),
                                  dict(P=256), dict(T=-1), dict(seq=A), dict(seq=A + 64), dict(n_out=A + 128),
-                                 dict(pages=1 << 28), dict(width=1 << 28)])
+                                 dict(pages=1 << 28), dict(width=1 << 28), dict(T=(1 << 30) + 1)])
 def test_page_plan_refuses(bad):
     assert _lib().mimo_moe_page_plan(*plan_args(**bad)) == EINVAL
 
@@ -50,7 +50,8 @@ def test_page_release_refuses(bad):
                                  dict(slots=None), dict(T=0), dict(nq=0), dict(nkv=0), dict(d=12), dict(dv=12),
                                  dict(rot=3), dict(rot=-2), dict(rot=194), dict(d=512, rot=258), dict(theta=0.0),
                                  dict(vs=-1.0), dict(vs=float("nan")), dict(pages=0), dict(P=100), dict(qkv=A + 8),
-                                 dict(q=A + 2), dict(k=A + 8), dict(v=A + 4)])
+                                 dict(q=A + 2), dict(k=A + 8), dict(v=A + 4), dict(T=2**31 - 1),
+                                 dict(nq=2**31 - 1), dict(nq=1 << 26, nkv=1 << 26), dict(nkv=1 << 23)])
 def test_paged_rope_store_refuses(bad):
     d = dict(qkv=A, T=4, nq=8, nkv=2, d=192, dv=128, rot=64, theta=1e4, vs=0.0, pos=A, slots=A, pages=8, P=16, q=A,
              k=A, v=A, status=None, stream=None)
@@ -61,7 +62,7 @@ def test_paged_rope_store_refuses(bad):
 @pytest.mark.parametrize("bad", [dict(cu=None), dict(seq=None), dict(plan=None), dict(R=0), dict(R=4097), dict(T=0),
                                  dict(nq=0), dict(nkv=0), dict(nkv=3), dict(nq=258, nkv=2), dict(window=-1),
                                  dict(keep=-1), dict(window=0, keep=4), dict(width=0), dict(P=8), dict(width=1 << 28),
-                                 dict(plan=A + 8), dict(nb=-1)])
+                                 dict(plan=A + 8), dict(nb=-1), dict(T=(1 << 30) + 1)])
 def test_paged_attention_plan_refuses(bad):
     L = _lib()
     d = dict(cu=A, seq=A, R=2, T=40, nq=8, nkv=2, window=128, keep=4, width=8, P=16, plan=A, nb=0, status=None,
@@ -80,7 +81,7 @@ def test_paged_attention_plan_refuses(bad):
                                  dict(scale=float("nan")), dict(window=-1), dict(keep=-1), dict(window=0, keep=4),
                                  dict(pages=0), dict(P=24), dict(width=0), dict(q=A + 8), dict(k=A + 2), dict(v=A + 8),
                                  dict(out=A + 16), dict(plan=A + 4), dict(ws=A + 16), dict(nb=-1), dict(wb=-1),
-                                 dict(pages=1 << 26, nq=256, nkv=128, T=1)])
+                                 dict(pages=1 << 26, nq=256, nkv=128, T=1), dict(T=2**31 - 1)])
 def test_paged_attention_refuses(bad):
     L = _lib()
     d = dict(q=A, k=A, v=A, sinks=None, table=A, width=8, R=2, T=40, nq=8, nkv=2, d=192, dv=128, scale=0.1, window=128,
