@@ -15,7 +15,6 @@ A step's token rows are its requests' new tokens, one request after another; row
 there is no CPU path."""
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
@@ -28,16 +27,15 @@ PAGE_SIZES = (16, 32, 64, 128)
 MAX_REQUESTS = 4096
 
 
-_HERE = contextlib.nullcontext()
-
-
-def _on(dev: torch.device):
-    """The context in which kernels launch on `dev` (nothing to do when it is the current device)."""
-    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(dev.index)   # current_stream(dev).cuda_stream without the object
+def _launch(dev: torch.device, where: str, fn, *args) -> None:
+    """fn(*args, current stream of dev), on dev."""
+    i = dev.index
+    if i != torch._C._cuda_getDevice():
+        with torch.cuda.device(i):
+            return _launch(dev, where, fn, *args)
+    rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))   # current_stream(dev).cuda_stream without the object
+    if rc:
+        check(rc, where)
 
 
 def _int32(t: torch.Tensor, name: str, shape, dev=None) -> torch.Tensor:
@@ -150,12 +148,10 @@ def page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Ten
     _int32(new_lens, "new_lens", (R,), dev)
     _int32(free_pages, "free_pages", free_pages.shape, dev)
     _int32(n_free, "n_free", (1,), dev)
-    with _on(dev):
-        check(lib().mimo_moe_page_plan(lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
-                                       out.width, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0],
-                                       out.page_size, tokens, out.cu_q.data_ptr(), out.seq_lens.data_ptr(),
-                                       out.n_free.data_ptr(), out.positions.data_ptr(), out.slots.data_ptr(),
-                                       out.status.data_ptr(), _stream(dev)), "page_plan")
+    _launch(dev, "page_plan", lib().mimo_moe_page_plan, lens.data_ptr(), new_lens.data_ptr(), R, block_table.data_ptr(),
+            out.width, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0], out.page_size, tokens,
+            out.cu_q.data_ptr(), out.seq_lens.data_ptr(), out.n_free.data_ptr(), out.positions.data_ptr(),
+            out.slots.data_ptr(), out.status.data_ptr())
     return out
 
 
@@ -174,11 +170,9 @@ def page_release(done: torch.Tensor, lens: torch.Tensor, block_table: torch.Tens
     _int32(lens, "lens", (R,), dev)
     _int32(free_pages, "free_pages", free_pages.shape, dev)
     _int32(n_free, "n_free", (1,), dev)
-    with _on(dev):
-        check(lib().mimo_moe_page_release(done.data_ptr(), R, lens.data_ptr(), block_table.data_ptr(),
-                                          block_table.shape[1], free_pages.data_ptr(), n_free.data_ptr(),
-                                          free_pages.shape[0], _page_size(page_size), _ptr(status), _stream(dev)),
-              "page_release")
+    _launch(dev, "page_release", lib().mimo_moe_page_release, done.data_ptr(), R, lens.data_ptr(),
+            block_table.data_ptr(), block_table.shape[1], free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0],
+            _page_size(page_size), _ptr(status))
 
 
 class _Rows:
@@ -310,12 +304,10 @@ def rope_store_paged(qkv: torch.Tensor, cfg: AttentionConfig, cache: PagedKVCach
     if T == 0:
         return q
     vs = 0.0 if cfg.v_scale is None else bf16_value(cfg.v_scale)
-    with _on(dev):
-        check(lib().mimo_moe_paged_rope_store(qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim,
-                                              cfg.v_head_dim, cfg.rotary_dim, float(cfg.rope_theta), vs,
-                                              step.positions.data_ptr(), step.slots.data_ptr(), cache.num_pages,
-                                              cache.page_size, q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(),
-                                              step.status.data_ptr(), _stream(dev)), "rope_store_paged")
+    _launch(dev, "rope_store_paged", lib().mimo_moe_paged_rope_store, qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads,
+            cfg.head_dim, cfg.v_head_dim, cfg.rotary_dim, cfg.rope_theta, vs, step.positions.data_ptr(),
+            step.slots.data_ptr(), cache.num_pages, cache.page_size, q.data_ptr(), cache.k.data_ptr(),
+            cache.v.data_ptr(), step.status.data_ptr())
     return q
 
 
@@ -337,17 +329,17 @@ class AttentionPlan:
         self.buffer, self._ws = None, {}
         if step.tokens == 0:
             return
-        with _on(step.device):
-            L = lib()
-            nb = L.mimo_moe_paged_attention_plan_bytes(step.tokens, step.requests, cfg.n_heads, cfg.n_kv_heads)
+        with torch.cuda.device(step.device):
+            nb = lib().mimo_moe_paged_attention_plan_bytes(step.tokens, step.requests, cfg.n_heads, cfg.n_kv_heads)
             self.buffer = torch.empty(nb, dtype=torch.uint8, device=step.device)
-            self.update()
+        self.update()
 
     def workspace_bytes(self, v_head_dim: int) -> int:
         nb = self._ws.get(v_head_dim)
         if nb is None:
-            nb = self._ws[v_head_dim] = lib().mimo_moe_paged_attention_workspace_bytes(
-                self.step.tokens, self.step.requests, self.kind[0], self.kind[1], v_head_dim)
+            with torch.cuda.device(self.step.device):
+                nb = self._ws[v_head_dim] = lib().mimo_moe_paged_attention_workspace_bytes(
+                    self.step.tokens, self.step.requests, self.kind[0], self.kind[1], v_head_dim)
         return nb
 
     def update(self) -> None:
@@ -355,11 +347,9 @@ class AttentionPlan:
         step, (nq, nkv, window, keep) = self.step, self.kind
         if self.buffer is None:
             return
-        with _on(step.device):
-            check(lib().mimo_moe_paged_attention_plan(step.cu_q.data_ptr(), step.seq_lens.data_ptr(), step.requests,
-                                                      step.tokens, nq, nkv, window, keep, step.width, step.page_size,
-                                                      self.buffer.data_ptr(), self.buffer.numel(),
-                                                      step.status.data_ptr(), _stream(step.device)), "attention_plan")
+        _launch(step.device, "attention_plan", lib().mimo_moe_paged_attention_plan, step.cu_q.data_ptr(),
+                step.seq_lens.data_ptr(), step.requests, step.tokens, nq, nkv, window, keep, step.width, step.page_size,
+                self.buffer.data_ptr(), self.buffer.numel(), step.status.data_ptr())
 
 
 def attention_plan(step: PageStep, cfg: AttentionConfig) -> AttentionPlan:
@@ -391,15 +381,13 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
         raise ValueError("attention_paged: the plan was made for another step or kind of layer")
     if T == 0:
         return o
-    with _on(dev):
-        nb = plan.workspace_bytes(cfg.v_head_dim)
-        ws = torch.empty(nb, dtype=torch.uint8, device=dev)   # the call's own: two streams or graphs never share it
-        check(lib().mimo_moe_paged_attention(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), _ptr(sinks),
-                                             step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,
-                                             cfg.n_kv_heads, cfg.head_dim, cfg.v_head_dim, float(cfg.scale),
-                                             cfg.window, cfg.keep_first, cache.num_pages, cache.page_size,
-                                             plan.buffer.data_ptr(), plan.buffer.numel(), o.data_ptr(), ws.data_ptr(),
-                                             nb, step.status.data_ptr(), _stream(dev)), "attention_paged")
+    nb = plan.workspace_bytes(cfg.v_head_dim)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)   # the call's own: two streams or graphs never share it
+    _launch(dev, "attention_paged", lib().mimo_moe_paged_attention, q.data_ptr(), cache.k.data_ptr(),
+            cache.v.data_ptr(), _ptr(sinks), step.block_table.data_ptr(), step.width, step.requests, T, cfg.n_heads,
+            cfg.n_kv_heads, cfg.head_dim, cfg.v_head_dim, cfg.scale, cfg.window, cfg.keep_first, cache.num_pages,
+            cache.page_size, plan.buffer.data_ptr(), plan.buffer.numel(), o.data_ptr(), ws.data_ptr(), nb,
+            step.status.data_ptr())
     return o
 
 
