@@ -29,7 +29,7 @@
 // cycles and more instructions took as long).  A tile's round of softmax (2000 cycles), P V and S (1420) and four
 // hand-overs is 4100 cycles and more, in which the tensor core works 2 x 1280.  Without any exponential it is still 3770;
 // two threads a row, two issuing warps, P in halves and a helper for the issuer's waits were all slower.  64 decoding
-// requests (580 MB of K and V) take 111 us, 5.2 TB/s; 8 of them at 4096 tokens (84 MB) 25 us, of which 9 pass before the
+// requests (580 MB of K and V) take 110 us, 5.3 TB/s; 8 of them at 4096 tokens (84 MB) 25 us, of which 9 pass before the
 // first product: the plan, the table, K and V come from HBM one after the other.
 #include <cstring>
 #include <type_traits>
@@ -868,18 +868,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       bool fresh = true;
       const float sink = p.sinks && row_ok ? p.sinks[g.hk * p.G + head] * kLog2e : 0.f;
       // where the row's output goes, worked out while the scores are on their way: itself, or a part in the workspace;
-      // and the rows of the quad's lanes, which exchange theirs
+      // and the rows of the pair of lanes that exchange theirs
       const int row = g.row0 + tt;
       const bool store = row_ok && row < p.T;
       const size_t at = part0 + (size_t)max(g.slot, 0) * part_rows + (tt * p.G + head);
       uint8_t* to = g.slot < 0 ? reinterpret_cast<uint8_t*>(p.out + ((size_t)row * p.nq + g.hk * p.G + head) * DV)
                                : reinterpret_cast<uint8_t*>(p.part_o + at * DV);
-      uint8_t* quad_to[4];
+      uint8_t* pair_to[2] = {to, to};
+      uint32_t pair_ok = 0;
+      if constexpr (LIST == kLarge) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        quad_to[k] = reinterpret_cast<uint8_t*>(
-            __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(to), (lane & ~3) | k));
-      const uint32_t quad_ok = __ballot_sync(0xFFFFFFFFu, store) >> (lane & ~3);
+        for (int k = 0; k < 2; ++k)
+          pair_to[k] = reinterpret_cast<uint8_t*>(
+              __shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(to), (lane & ~1) | k));
+        pair_ok = __ballot_sync(0xFFFFFFFFu, store) >> (lane & ~1);
+      }
       // after a wait that ran out the loops go on without work, for the barriers that both groups must pass
       for (int j = pair ? 0 : x; j < g.nblk; j += pair ? 1 : 2) {
         if (ok) ok = mbar_wait(&s_full[x], ns & 1);
@@ -1040,58 +1043,57 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
           }
         }
         w_own *= f, w_other *= f;
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 32) {
-          float o[32];
-          tmem_ld32(tO + c, o);
-          if (pair) {
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= w_own;
-          } else {
-            float q[32];
-            tmem_ld32(tOther + c, q);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              o[e] = own ? o[e] * w_own : 0.f;
-              o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
-            }
-          }
+        // 32 columns of the warp's rows: 64 bytes of a row, stored as whole sectors.  A store to 32 different rows takes
+        // the load/store unit 32 turns; with eight warps at it, lanes of a pair first exchange theirs, so that a store
+        // writes 64 bytes of 16 rows (23 decoding requests + 2 chunks: 113.5 us instead of 117.0).  A small unit's one
+        // warp a tile is better off without the shuffles (48 requests in a window of 128: 18.1 us instead of 19.1).
+        auto emit = [&](int c, float* o) {
           if (g.slot >= 0) {
             if (store)
 #pragma unroll
               for (int e = 0; e < 32; e += 8)
                 st_global_v8(reinterpret_cast<float*>(to) + c + e, reinterpret_cast<uint32_t*>(o + e));
-            continue;
+            return;
           }
-          // The 32 columns are 64 bytes of a row.  A store of a piece of 32 different rows takes the load/store unit 32
-          // turns, so the four lanes of a quad first exchange theirs: the 16 bytes q of the quad's rows go to lane q, and a
-          // store writes 64 bytes of 8 rows.
           uint32_t w[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) w[e] = pack_bf16x2_rn(o[2 * e], o[2 * e + 1]);
-#pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const bool hi = (lane >> st) & 1;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if ((k >> st) & 1) continue;
-              const int k1 = k | (1 << st);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t give = hi ? w[k * 4 + e] : w[k1 * 4 + e];
-                const uint32_t take = __shfl_xor_sync(0xFFFFFFFFu, give, 1 << st);
-                w[k * 4 + e] = hi ? take : w[k * 4 + e];
-                w[k1 * 4 + e] = hi ? w[k1 * 4 + e] : take;
-              }
+          if constexpr (LIST == kSmall) {
+            if (store) {
+              st_global_v8(to + c * 2, w);
+              st_global_v8(to + c * 2 + 32, w + 8);
             }
-          }
+          } else {
+            const bool odd = lane & 1;
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if ((quad_ok >> k) & 1)
-              *reinterpret_cast<uint4*>(quad_to[k] + c * 2 + (lane & 3) * 16) =
-                  make_uint4(w[k * 4], w[k * 4 + 1], w[k * 4 + 2], w[k * 4 + 3]);
+            for (int e = 0; e < 8; ++e) {
+              const uint32_t take = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[e] : w[8 + e], 1);
+              w[e] = odd ? take : w[e];
+              w[8 + e] = odd ? w[8 + e] : take;
+            }
+            if (pair_ok & 1) st_global_v8(pair_to[0] + c * 2 + odd * 32, w);
+            if (pair_ok & 2) st_global_v8(pair_to[1] + c * 2 + odd * 32, w + 8);
+          }
+        };
+#pragma unroll 1
+        for (int c = c0; c < c1; c += pair ? 64 : 32) {  // 64 columns at a time, or 32 of both outputs
+          float o[32], q[32];
+          tmem_ld32(tO + c, o);
+          tmem_ld32(pair ? tO + c + 32 : tOther + c, q);
+          tc::tmem_wait_ld();
+          if (pair) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= w_own, q[e] *= w_own;
+            emit(c, o);
+            emit(c + 32, q);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              o[e] = own ? o[e] * w_own : 0.f;
+              o[e] = other ? fmaf(q[e], w_other, o[e]) : o[e];
+            }
+            emit(c, o);
+          }
         }
         if (store && g.slot >= 0 && c0 == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(m_ref, l);
       }
