@@ -29,7 +29,7 @@
 // cycles and more instructions took as long).  A tile's round of softmax (2000 cycles), P V and S (1420) and four
 // hand-overs is 4100 cycles and more, in which the tensor core works 2 x 1280.  Without any exponential it is still 3770;
 // two threads a row, two issuing warps, P in halves and a helper for the issuer's waits were all slower.  64 decoding
-// requests (580 MB of K and V) take 110 us, 5.3 TB/s; 8 of them at 4096 tokens (84 MB) 25 us, of which 9 pass before the
+// requests (580 MB of K and V) take 107 us, 5.4 TB/s; 8 of them at 4096 tokens (84 MB) 23 us, of which 9 pass before the
 // first product: the plan, the table, K and V come from HBM one after the other.
 #include <cstring>
 #include <type_traits>
@@ -462,17 +462,23 @@ constexpr uint32_t kHead = 1024 + 2048;  // barriers, the exchange between the s
 constexpr uint32_t kChunk = 16384;  // 128 positions x 64 dims, bf16
 
 // Shared memory of the kernel of each list.  A tile of the MMA is 128 rows either way; a small unit's Q is only
-// kSmallRows of them in memory (the MMA reads what lies behind for the others, and nobody reads their results), which
-// leaves the ring of K and V room for what HBM's latency needs in flight: with the ring that two whole Q tiles leave, a
-// decoding request's block took 2.5 us, most of it the wait for K.
+// kSmallRows of them in memory, which leaves the ring of K and V room for what HBM's latency needs in flight: with the
+// ring that two whole Q tiles leave, a decoding request's block took 2.5 us, most of it the wait for K.  For the other
+// rows the MMA reads what lies behind: zeros, after the second buffer's the first one's rows and then zeros (nobody reads
+// these results, but products of zeros take less power: with a ring of 12 slots and other data behind Q, 64 decoding
+// requests took 125 us under the power cap instead of 117, and 8 of them 24.8 instead of 23.2).
 template <int DQK, int DV, int LIST>
 struct Shape {
   static constexpr int QCH = DQK / 64, VCH = DV / 64;
-  static constexpr uint32_t QCHUNK = (LIST == kSmall ? kSmallRows : 128) * 128u;  // 64 dims of a Q tile
-  static constexpr uint32_t QB = QCH * QCHUNK;
+  static constexpr uint32_t QROWS = (LIST == kSmall ? kSmallRows : 128) * 128u;  // the rows of 64 dims of a Q tile
+  static constexpr uint32_t QZERO = LIST == kSmall ? 128 * 128u - QROWS : 0;    // and the zeros behind both buffers'
+  static constexpr uint32_t QB = QCH * (2 * QROWS + QZERO);
+  static constexpr __host__ __device__ uint32_t q_at(int buffer, int chunk) {
+    return chunk * (2 * QROWS + QZERO) + (1 - buffer) * QROWS;
+  }
   static constexpr int NG = 16;  // barriers of K and V blocks: more than the ring holds
-  static constexpr int NS = (int)((232448u - kHead - 2 * QB) / kChunk);  // ring slots in what Q leaves
-  static constexpr uint32_t SMEM = kHead + 2 * QB + NS * kChunk;
+  static constexpr int NS = (int)((232448u - kHead - QB) / kChunk);  // ring slots in what Q leaves
+  static constexpr uint32_t SMEM = kHead + QB + NS * kChunk;
   // a single tile's second K block is read before its first V block leaves the ring
   static_assert(2 * QCH + VCH <= NS, "the ring must hold K, V and the next K");
   static_assert(2 * ((NS + QCH + VCH - 1) / (QCH + VCH)) < NG, "a barrier for every block in the ring");
@@ -502,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
   volatile uint32_t* issuer_gone = tslot + 1;  // a wait of the MMA issuer ran out
   float2* xchg = reinterpret_cast<float2*>(smem + 1024);  // [2][128] (maximum, sum) of the tiles' rows
   uint8_t* sQ = smem + kHead;
-  uint8_t* sRing = sQ + 2 * S::QB;
+  uint8_t* sRing = sQ + S::QB;
   if (smem_u32(smem) & 1023) {  // never seen: the swizzled tiles would be read wrongly
     if (threadIdx.x == 0) set_status(p.status, MIMO_EINVAL);
     return;
@@ -528,6 +534,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
     mbar_init(drain, 1);
     *issuer_gone = 0;
     mbar_fence_init();
+  }
+  if constexpr (LIST == kSmall) {
+    for (int c = 0; c < S::QCH; ++c)
+      for (uint32_t i = threadIdx.x * 16; i < S::QZERO; i += kThreads * 16)
+        *reinterpret_cast<uint4*>(sQ + S::q_at(0, c) + S::QROWS + i) = make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async_smem();
   }
   if (warp == 9) {
     tc::tmem_alloc(tslot, 512);
@@ -636,7 +648,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
               mbar_arrive_expect_tx(&q_full[qb], (uint32_t)(S::QCH * 128 * p.G * tpt));
 #pragma unroll
               for (int d = 0; d < S::QCH; ++d)
-                tma_box(sQ + qb * S::QB + d * S::QCHUNK, &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[qb]);
+                tma_box(sQ + S::q_at(qb, d), &p.qmap, d * 64, g.hk * p.G, g.row0 + x * tpt, &q_full[qb]);
             }
           }
           if (!pair) turn ^= 1;
@@ -698,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
         if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < S::QCH; ++c) {
-            const uint32_t a = aq + (qb * S::QB + c * S::QCHUNK) / 16, b = bk + wrap(at + c) * (kChunk / 16);
+            const uint32_t a = aq + S::q_at(qb, c) / 16, b = bk + wrap(at + c) * (kChunk / 16);
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk) mma_ss(d, a + kk * 2, b + kk * 2, idesc_s, (c | kk) != 0);
           }
