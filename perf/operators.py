@@ -11,22 +11,12 @@ ones; the step's token rows are the requests' new tokens one request after anoth
 
 `own` false: elementary torch operations.  `own` true: the calls a user makes."""
 import math
-import os
 import random
-import sys
 
 import numpy as np
 import torch
 
 own = False
-PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mimo-on-a-mac_b200")
-
-
-def _framework():
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
-    from mimo_moe import layer, paged
-    return layer, paged
 
 # Attention shapes: the full-attention and sliding-window layers of this repository's default configuration, and the
 # two other head layouts its attention tests use.
@@ -190,7 +180,7 @@ def prepare(case, seed):
         s.update(lens=held_t, new_lens=new_t, free=free,
                  n_free=torch.full((1,), num_pages - used, dtype=torch.int32, device=dev))
         if own:
-            _, paged = _framework()
+            from mimo_moe import paged
             s["step"] = paged.PageStep.empty(R, T, table, P)
         return s
     k = KINDS[case["kind"]]
@@ -217,10 +207,11 @@ def prepare(case, seed):
         s["sinks"] = torch.randn(nq, generator=g, device=dev) if k["sinks"] else None
         s["out"] = torch.zeros(T, nq, dv, dtype=torch.bfloat16, device=dev)
     if own:
-        layer, paged = _framework()
+        from mimo_moe import paged
+        from mimo_moe.layer import AttentionConfig
         keep = case["keep"] if case["op"] == "attn" else 0
-        s["cfg"] = layer.AttentionConfig(**k, v_scale=V_SCALE if case["op"] == "rope" and k["window"] else None,
-                                         keep_first=keep)
+        s["cfg"] = AttentionConfig(**k, v_scale=V_SCALE if case["op"] == "rope" and k["window"] else None,
+                                   keep_first=keep)
         s["cache"] = paged.PagedKVCache(s["cfg"], num_pages, P, k=s["k"], v=s["v"])
         s["step"] = paged.PageStep(block_table=table, page_size=P, cu_q=cu, seq_lens=seq_lens, positions=pos,
                                    slots=slots)
@@ -232,7 +223,7 @@ def prepare(case, seed):
 def run(s):
     op = s["case"]["op"]
     if own:
-        _, paged = _framework()
+        from mimo_moe import paged
         if op == "plan":
             p = paged.page_plan(s["lens"], s["new_lens"], s["table"], s["free"], s["n_free"], s["page"], s["tokens"],
                                 out=s["step"])
