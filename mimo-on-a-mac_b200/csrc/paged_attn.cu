@@ -601,20 +601,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attn_kernel(const __grid_co
       const int qlast = g.qfirst + g.ntok - 1;
       const Blocks bl = blocks_of(g.qfirst, qlast, p.window, p.keep);
       const int* trow = p.table + (size_t)g.r * p.width;
-      // the number of the block's page `lane`, num_pages for one nobody sees; loaded a block ahead
-      auto page_of = [&](int j) -> int {
+      // the number of the block's page `lane`, and whether a query sees that page (a flag of its own: the table may hold
+      // any number); loaded a block ahead
+      int page = 0;
+      bool vis = false;
+      auto load_page = [&](int j) {
         const int kb = j < bl.nkb ? j : bl.lb + (j - bl.nkb);
         const int pg = kb * ppb + lane, pos = pg << p.page_shift;
-        if (lane >= ppb || pg >= p.width || pos > qlast || (pos + P - 1 < bl.lo && pos >= bl.keep)) return p.num_pages;
-        return trow[pg];
+        vis = lane < ppb && pg < p.width && pos <= qlast && (pos + P - 1 >= bl.lo || pos < bl.keep);
+        if (vis) page = trow[pg];
       };
-      int page = page_of(g.b0);
+      load_page(g.b0);
       for (int j = 0; j < g.nblk && ok; ++j) {
-        int row = nowhere;
-        if ((unsigned)page < (unsigned)p.num_pages) row = page * p.nkv + g.hk;
-        else if (page != p.num_pages) set_status(p.status, MIMO_ERANGE);
-        const uint32_t seen = __ballot_sync(0xFFFFFFFFu, page != p.num_pages);
-        if (j + 1 < g.nblk) page = page_of(g.b0 + j + 1);
+        const bool in_pool = (unsigned)page < (unsigned)p.num_pages;
+        const int row = in_pool ? page * p.nkv + g.hk : nowhere;
+        if (vis && !in_pool) set_status(p.status, MIMO_ERANGE);
+        const uint32_t seen = __ballot_sync(0xFFFFFFFFu, vis);
+        if (j + 1 < g.nblk) load_page(g.b0 + j + 1);
         int rows[8];  // the same in all lanes: uniform registers, from which a copy is issued in 25 cycles
 #pragma unroll
         for (int i = 0; i < 8; ++i) rows[i] = __shfl_sync(0xFFFFFFFFu, row, i);

@@ -734,3 +734,26 @@ def test_attention_paged_in_a_call_of_seconds(gpu):
     K, V = cache.k[0].transpose(0, 1).cpu(), cache.v[0].transpose(0, 1).cpu()
     for k in (1, 1000, T // P):
         compare(cfg, out[k * P - 1:k * P], q[k * P - 1:k * P].cpu(), [(K, V)], [P - 1], [1], None, blocks=k)
+
+
+@pytest.mark.parametrize("number", [lambda n: n, lambda n: n + 1, lambda n: 2**31 - 1, lambda n: -1, lambda n: -2**31],
+                         ids=["n", "n + 1", "largest", "-1", "smallest"])
+@pytest.mark.parametrize("dims", [D128, dict(SWA, window=400, keep_first=40)], ids=["full", "window"])
+def test_attention_paged_reads_a_page_outside_the_pool_as_zeros(gpu, dims, number):
+    """Every page number that is none of the pool's, the first one behind it among them: an error, and zeros for k and v,
+    in a decoding request, a prompt's chunk and a split unit."""
+    from mimo_moe import paged
+    cfg = cfg_of(dims)
+    held, new, P = [900, 600, 70, 9000], [1, 200, 1, 1], 16
+    step, cache, q, kv, sinks = fill(cfg, held, new, P, gpu, 12)
+    paged.attention_paged(q.to(gpu), cache, cfg, step, sinks)
+    step.check()
+    for r, pages in ((0, (0, 41, 55)), (1, (2, 30, 49)), (3, (1, 550, 562))):
+        for j in pages:
+            step.block_table[r, j] = number(cache.num_pages)
+            for t in kv[r]:
+                t[j * P:(j + 1) * P] = 0.0
+    out = paged.attention_paged(q.to(gpu), cache, cfg, step, sinks)
+    with pytest.raises(ValueError):
+        step.check()
+    compare(cfg, out, q, kv, held, new, sinks)
