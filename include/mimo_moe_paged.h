@@ -61,6 +61,14 @@ int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_hea
                               float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
                               int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages, int32_t* status,
                               void* stream);
+/* The same, and the rows of `clear` (bf16 [tokens][clear_width], clear_width a multiple of 8) whose slot is negative
+ * become zero: for the `out` of the attention that follows, which leaves padding rows as they are, when all of its rows
+ * go on into the layer.  clear may be null. */
+int mimo_moe_paged_rope_store_clear(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                                    int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,
+                                    float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
+                                    int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages,
+                                    uint16_t* clear, int32_t clear_width, int32_t* status, void* stream);
 
 /* Attention of the step's new tokens over the paged cache (k and v of the new tokens already stored): row
  * cu_q[r] + i of request r is the query at position p = seq_lens[r] - (cu_q[r + 1] - cu_q[r]) + i and sees the key

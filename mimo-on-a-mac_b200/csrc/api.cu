@@ -1187,24 +1187,36 @@ int mimo_moe_page_release(const uint8_t* done, int32_t R, int32_t* lens, int32_t
   return MIMO_OK;
 }
 
-int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
-                              int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,
-                              float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
-                              int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages, int32_t* status,
-                              void* stream) {
+int mimo_moe_paged_rope_store_clear(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                                    int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,
+                                    float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
+                                    int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages,
+                                    uint16_t* clear, int32_t clear_width, int32_t* status, void* stream) {
   if (!qkv || !positions || !slots || !q || !k_pages || !v_pages || tokens < 1 || tokens > kMaxTokens || n_heads < 1 ||
       n_kv_heads < 1 || head_dim < 8 || v_head_dim < 8 || head_dim % 8 || v_head_dim % 8 || rotary_dim < 0 || rotary_dim % 2 ||
       rotary_dim > head_dim || rotary_dim > 256 ||
       ((int64_t)n_heads + n_kv_heads) * head_dim + (int64_t)n_kv_heads * v_head_dim > kMaxTokens || !(rope_theta > 0.f) || !(v_scale >= 0.f) ||
-      bad_pool(num_pages, page_size) || !a16(qkv) || !a16(q) || !a16(k_pages) || !a16(v_pages))
+      bad_pool(num_pages, page_size) || !a16(qkv) || !a16(q) || !a16(k_pages) || !a16(v_pages) ||
+      (clear != nullptr && (clear_width < 8 || clear_width % 8 || clear_width > kMaxTokens || !a16(clear))))
     return MIMO_EINVAL;
   PagedRopeParams p{};
   p.qkv = qkv, p.positions = positions, p.slots = slots, p.q = q, p.k = k_pages, p.v = v_pages, p.status = status;
+  p.clear = reinterpret_cast<uint4*>(clear), p.clear_n = clear_width / 8;
   p.T = tokens, p.nq = n_heads, p.nkv = n_kv_heads, p.dqk = head_dim, p.dv = v_head_dim, p.rot = rotary_dim;
   p.num_pages = num_pages, p.page_shift = page_shift_of(page_size), p.has_vscale = v_scale > 0.f ? 1 : 0;
   p.v_scale = v_scale, p.log_base = std::log((double)rope_theta);
   MIMO_TRY(launch_paged_rope(p, static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
+}
+
+int mimo_moe_paged_rope_store(const uint16_t* qkv, int32_t tokens, int32_t n_heads, int32_t n_kv_heads,
+                              int32_t head_dim, int32_t v_head_dim, int32_t rotary_dim, float rope_theta,
+                              float v_scale, const int32_t* positions, const int32_t* slots, int32_t num_pages,
+                              int32_t page_size, uint16_t* q, uint16_t* k_pages, uint16_t* v_pages, int32_t* status,
+                              void* stream) {
+  return mimo_moe_paged_rope_store_clear(qkv, tokens, n_heads, n_kv_heads, head_dim, v_head_dim, rotary_dim, rope_theta,
+                                         v_scale, positions, slots, num_pages, page_size, q, k_pages, v_pages, nullptr, 0,
+                                         status, stream);
 }
 
 namespace {

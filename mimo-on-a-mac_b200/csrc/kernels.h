@@ -339,6 +339,8 @@ struct PagedRopeParams {
   const uint16_t* qkv;               // [T][nq*dqk + nkv*dqk + nkv*dv] projection rows
   const int32_t *positions, *slots;  // [T], slot -1: not a token
   uint16_t *q, *k, *v;               // q [T][nq][dqk], pools [num_pages][nkv][page][d]
+  uint4* clear;                      // [T][clear_n] rows that become zero where the slot is -1, or null
+  int clear_n;
   int32_t* status;
   int T, nq, nkv, dqk, dv, rot, num_pages, page_shift, has_vscale;
   float v_scale;    // already a bf16 value

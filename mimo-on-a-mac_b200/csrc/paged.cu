@@ -260,7 +260,11 @@ __global__ void __launch_bounds__(THREADS) paged_rope_rows_kernel(PagedRopeParam
   for (; t < p.T; t += gridDim.x) {
     const int my_slot = slot, my_pos = pos;
     if (t + (int)gridDim.x < p.T) slot = p.slots[t + gridDim.x], pos = p.positions[t + gridDim.x];
-    if (my_slot < 0) continue;
+    if (my_slot < 0) {
+      if (p.clear != nullptr)
+        for (int i = tid; i < p.clear_n; i += THREADS) p.clear[(size_t)t * p.clear_n + i] = make_uint4(0, 0, 0, 0);
+      continue;
+    }
     if (tid < 32) {
       asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // the row before has left
       __syncwarp();
@@ -332,7 +336,12 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(PagedRopeParam
   pdl_wait();  // the projection rows and the plan come from preceding kernels (programmatic dependent launch)
   pdl_launch_dependents();
   const int slot = p.slots[t];
-  if (slot < 0) return;
+  if (slot < 0) {
+    if (p.clear != nullptr)
+      for (int i = blockIdx.y * kRopeThreads + tid; i < p.clear_n; i += gridDim.y * kRopeThreads)
+        p.clear[(size_t)t * p.clear_n + i] = make_uint4(0, 0, 0, 0);
+    return;
+  }
   if (tid < half) cs[tid] = rotary((double)p.positions[t] * freq[tid]);
   __syncthreads();
   const int page = slot >> p.page_shift, at = slot & ((1 << p.page_shift) - 1);

@@ -106,6 +106,9 @@ SIGNATURES = {
     "mimo_moe_paged_rope_store": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
                                             c_float, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                             c_void_p, c_void_p]),
+    "mimo_moe_paged_rope_store_clear": (c_int32, [c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_float,
+                                                  c_float, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                                                  c_void_p, c_void_p, c_int32, c_void_p, c_void_p]),
     "mimo_moe_paged_attention_plan_bytes": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "mimo_moe_paged_attention_plan": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32,
                                                 c_int32, c_int32, c_void_p, c_size_t, c_void_p, c_void_p]),

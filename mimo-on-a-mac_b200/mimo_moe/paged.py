@@ -268,8 +268,7 @@ class PagedKVCache:
 
     def attend(self, qkv: torch.Tensor, sinks: Optional[torch.Tensor]) -> torch.Tensor:
         """The layer's cache half (RoPE + append, attention) for the projection rows of `step`'s tokens.  The result is
-        the step's scratch, which the next layer's call writes again; its padding rows hold zeros or an earlier call's
-        values: finite, and nothing anyone asks for."""
+        the step's scratch, which the next layer's call writes again; its padding rows are zero."""
         step, cfg = self.step, self.cfg
         if step is None:
             raise ValueError("PagedKVCache: no step set (cache.step = table.step(new_lens, tokens))")
@@ -278,7 +277,7 @@ class PagedKVCache:
             return torch.zeros(n, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=self.device)
 
         out = step.rows.get(("attention", cfg.n_heads, cfg.v_head_dim), step.tokens, rows)
-        q = rope_store_paged(qkv, cfg, self, step)
+        q = rope_store_paged(qkv, cfg, self, step, clear=out)
         return attention_paged(q, self, cfg, step, sinks, plan=self.plan, out=out)
 
 
@@ -293,21 +292,24 @@ def _fits(cache: PagedKVCache, cfg: AttentionConfig, step: PageStep, where: str)
 
 
 def rope_store_paged(qkv: torch.Tensor, cfg: AttentionConfig, cache: PagedKVCache, step: PageStep,
-                     q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     q_out: Optional[torch.Tensor] = None, clear: Optional[torch.Tensor] = None) -> torch.Tensor:
     """mimo_moe.layer.rope_store for a step's token rows: RoPE on q and k at each row's position, v * the value scale,
-    k and v to each row's cache slot.  Returns q bf16 [tokens, n_heads, head_dim]; padding rows are not written."""
+    k and v to each row's cache slot.  Returns q bf16 [tokens, n_heads, head_dim]; padding rows are not written.  clear:
+    the attention's `out` (bf16 [tokens, n_heads, v_head_dim]), whose padding rows (those without a slot) become zero."""
     _fits(cache, cfg, step, "rope_store_paged")
     T, dev = step.tokens, step.device
     qkv = _bf16(qkv, "qkv", (T, cfg.qkv_width), dev)
     shape = (T, cfg.n_heads, cfg.head_dim)
     q = torch.empty(shape, dtype=torch.bfloat16, device=dev) if q_out is None else _buffer(q_out, "q_out", shape, dev)
+    if clear is not None:
+        _buffer(clear, "clear", (T, cfg.n_heads, cfg.v_head_dim), dev)
     if T == 0:
         return q
     vs = 0.0 if cfg.v_scale is None else bf16_value(cfg.v_scale)
-    _launch(dev, "rope_store_paged", lib().mimo_moe_paged_rope_store, qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads,
+    _launch(dev, "rope_store_paged", lib().mimo_moe_paged_rope_store_clear, qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads,
             cfg.head_dim, cfg.v_head_dim, cfg.rotary_dim, cfg.rope_theta, vs, step.positions.data_ptr(),
             step.slots.data_ptr(), cache.num_pages, cache.page_size, q.data_ptr(), cache.k.data_ptr(),
-            cache.v.data_ptr(), step.status.data_ptr())
+            cache.v.data_ptr(), _ptr(clear), cfg.n_heads * cfg.v_head_dim, step.status.data_ptr())
     return q
 
 

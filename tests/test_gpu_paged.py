@@ -757,3 +757,81 @@ def test_attention_paged_reads_a_page_outside_the_pool_as_zeros(gpu, dims, numbe
     with pytest.raises(ValueError):
         step.check()
     compare(cfg, out, q, kv, held, new, sinks)
+
+
+def attend_steps(gpu, dims, R=6, P=16):
+    """A cache, its table and a function that runs attend on a step of given new lengths (rows of NaN where said)."""
+    from mimo_moe import paged
+    cfg = cfg_of(dims)
+    sinks = torch.zeros(cfg.n_heads, device=gpu) if cfg.sinks else None
+    table = paged.PageTable(R, 512, 80, P, gpu)
+    cache = paged.PagedKVCache(cfg, 80, P, gpu)
+
+    def run(new, rows, nan=()):
+        qkv = torch.randn(rows, cfg.qkv_width, device=gpu, generator=torch.Generator(gpu).manual_seed(rows))
+        for r in nan:
+            qkv[r] = float("nan")
+        cache.step = table.step(i32(new, gpu), rows)
+        return cache.attend(qkv, sinks)
+
+    return run, table, cache, sinks
+
+
+@pytest.mark.parametrize("dims", [FULL, dict(SWA, rotary_dim=34), D64], ids=["full", "window, odd rotary", "d64"])
+def test_padding_rows_of_a_layer_are_zero_whatever_the_rows_held_before(gpu, dims):
+    """A request's NaN stays its own: the next, shorter step has zeros in the rows that held it."""
+    run, table, cache, _ = attend_steps(gpu, dims)
+    out = run([100, 2, 2, 0, 0, 30], 140, nan=range(104, 140))
+    assert torch.isnan(out[104:134]).any() and torch.isfinite(out[:104]).all() and (out[134:] == 0).all()
+    out = run([1, 0, 1, 0, 0, 0], 140)
+    assert torch.isfinite(out[:2]).all() and (out[:2] != 0).any() and (out[2:] == 0).all()
+    out = run([0] * 6, 140)
+    assert (out == 0).all()
+    cache.step.check()
+
+
+def test_padding_rows_are_zero_in_a_buffer_that_a_capture_made(gpu):
+    """A buffer made while a graph is captured lies in memory that an earlier graph left full of NaN; an eager padded
+    step uses it before the graph's first replay, another one after."""
+    run, table, cache, sinks = attend_steps(gpu, FULL)
+    run([1, 1, 1, 1, 1, 1], 6)
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        torch.full((1 << 24,), float("nan"), device=gpu)
+    first.replay()
+    rows = 64
+    qkv = torch.randn(rows, cache.cfg.qkv_width, device=gpu, dtype=torch.bfloat16)
+    new = i32([1, 2, 3, 4, 5, 6], gpu)
+    with torch.cuda.graph(second, pool=first.pool()):
+        cache.step = table.step(new, rows)
+        got = cache.attend(qkv, sinks)
+    assert (run([1, 0, 1, 0, 0, 0], rows)[2:] == 0).all()
+    second.replay()
+    assert (got[:21] != 0).any() and (got[21:] == 0).all()
+    assert (run([1, 0, 1, 0, 0, 0], rows)[2:] == 0).all()
+    cache.step.check()
+
+
+def test_padding_rows_of_a_paged_stack_stay_finite(gpu):
+    from mimo_moe.paged import PagedDecoderStack
+    stack = PagedDecoderStack(stack_layers(gpu), max_requests=3, max_len=256, num_pages=40, page_size=16)
+    x = torch.randn(40, 1024, device=gpu).to(torch.bfloat16)
+    x[30:] = float("nan")
+    assert torch.isnan(stack(x, i32([20, 10, 10], gpu))[30:]).all()
+    x = torch.zeros(40, 1024, device=gpu, dtype=torch.bfloat16)
+    assert torch.isfinite(stack(x, i32([1, 1, 0], gpu))).all()
+    stack.check()
+
+
+def test_rope_store_paged_refuses_another_clear(gpu):
+    from mimo_moe import paged
+    cfg = cfg_of(D64)
+    step, _, N = layout([0], [4], 16, gpu, 2)
+    cache = paged.PagedKVCache(cfg, N, 16, gpu)
+    qkv = torch.zeros(4, cfg.qkv_width, dtype=torch.bfloat16, device=gpu)
+    good = torch.zeros(4, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=gpu)
+    paged.rope_store_paged(qkv, cfg, cache, step, clear=good)
+    for bad in (good[:3], good.float(), good.cpu(), good[:, :4], torch.zeros(4, 16, 64, dtype=torch.bfloat16,
+                                                                             device=gpu)[:, ::2]):
+        with pytest.raises(ValueError):
+            paged.rope_store_paged(qkv, cfg, cache, step, clear=bad)

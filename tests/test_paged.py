@@ -120,3 +120,12 @@ def test_ring_attention_refuses_first_tokens_that_stay():
     cfg = AttentionConfig(window=128, keep_first=4)
     with pytest.raises(ValueError):
         attention(torch.zeros(1, 64, 192), KVCache(cfg, 128, "cpu"), cfg, 0)
+
+
+@pytest.mark.parametrize("bad", [dict(clear=A + 8), dict(width=0), dict(width=-8), dict(width=12), dict(width=(1 << 30) + 8),
+                                 dict(q=None), dict(clear=A, T=0)])
+def test_paged_rope_store_clear_refuses(bad):
+    d = dict(qkv=A, T=4, nq=8, nkv=2, d=192, dv=128, rot=64, theta=1e4, vs=0.0, pos=A, slots=A, pages=8, P=16, q=A,
+             k=A, v=A, clear=A, width=1024, status=None, stream=None)
+    d.update(bad)
+    assert _lib().mimo_moe_paged_rope_store_clear(*d.values()) == EINVAL
