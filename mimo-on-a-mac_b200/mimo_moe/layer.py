@@ -64,6 +64,11 @@ def bf16_value(v: float) -> float:
     return float(torch.tensor(v, dtype=torch.float32).to(torch.bfloat16).to(torch.float32))
 
 
+def _no_keep_first(cfg: AttentionConfig, where: str) -> None:
+    if cfg.keep_first:
+        raise ValueError(f"{where}: a ring cache no longer holds the first tokens (keep_first needs a paged cache)")
+
+
 class KVCache:
     """Device KV cache of one attention layer: k [n_kv, cap, head_dim], v [n_kv, cap, v_head_dim] bf16,
     position p in slot p % cap.  Full attention: cap = the longest sequence (mlx_lm KVCache); sliding window:
@@ -73,6 +78,7 @@ class KVCache:
     paged = False   # one sequence, as against mimo_moe.paged.PagedKVCache
 
     def __init__(self, cfg: AttentionConfig, cap: int, device=None):
+        _no_keep_first(cfg, "KVCache")
         dev = torch.device(device or "cuda")
         self.cfg = cfg
         self.cap = int(cap)
@@ -113,8 +119,7 @@ def attention(q: torch.Tensor, cache: KVCache, cfg: AttentionConfig, pos0: int, 
     rows run on the tcgen05 kernel (cache capacity a multiple of 128), decode-sized calls on the split-key
     mma.sync kernel.  Returns bf16 [T, n_heads, v_head_dim]."""
     _need_cuda(q, "q")
-    if cfg.keep_first:
-        raise ValueError("attention: a ring cache no longer holds the first tokens (keep_first needs a paged cache)")
+    _no_keep_first(cfg, "attention")
     q = q.to(torch.bfloat16).contiguous()
     T = q.shape[0]
     dev = q.device
@@ -226,8 +231,9 @@ class Attention:
         cfg = self.cfg
         if cache.paged:   # rows of many requests, laid out by the cache's step
             return linear(cache.attend(linear(r, self.w_qkv), self.sinks).view(T, -1), self.w_o)
+        _no_keep_first(cfg, "attention")
         # the attention call's own check (every key visible to the chunk still in the ring), made before the
-        # cache append so a refused chunk leaves the cache as it was
+        # cache append (as the one above) so a refused chunk leaves the cache as it was
         first = max(0, cache.offset - cfg.window + 1) if cfg.window > 0 else 0
         need = cache.offset + T - first
         if need > cache.cap:

@@ -129,3 +129,21 @@ def test_paged_rope_store_clear_refuses(bad):
              k=A, v=A, clear=A, width=1024, status=None, stream=None)
     d.update(bad)
     assert _lib().mimo_moe_paged_rope_store_clear(*d.values()) == EINVAL
+
+
+def test_first_tokens_that_stay_are_refused_before_a_ring_cache_is_touched():
+    """By the cache itself, and by a layer given one that was made for another config, before it appends."""
+    from mimo_moe.layer import Attention, AttentionConfig, DecoderLayer, DecoderStack, KVCache
+    plain = AttentionConfig(n_heads=2, n_kv_heads=1, head_dim=64, v_head_dim=64, rotary_dim=32, window=128)
+    cfg = AttentionConfig(n_heads=2, n_kv_heads=1, head_dim=64, v_head_dim=64, rotary_dim=32, window=128, keep_first=4)
+    w = torch.zeros(128, 256, dtype=torch.bfloat16)
+    attn = Attention(cfg, w, w[:64], w[:64], w.t())
+    for make in (lambda: KVCache(cfg, 256, "cpu"), lambda: KVCache.for_layer(cfg, 256, device="cpu"),
+                 lambda: DecoderLayer(attn, None, None, None).new_cache(256),
+                 lambda: DecoderStack([DecoderLayer(attn, None, None, None)], 256)):
+        with pytest.raises(ValueError, match="keep_first"):
+            make()
+    ring = KVCache(plain, 256, "cpu")
+    with pytest.raises(ValueError, match="keep_first"):
+        attn(torch.zeros(1, 256, dtype=torch.bfloat16), ring)
+    assert ring.offset == 0 and not ring.k.any()
