@@ -75,8 +75,6 @@ class KVCache:
     a ring of window + max_chunk - 1 slots (RotatingKVCache(max_size=window) keeps the last `window` keys and
     concatenates a multi-token chunk before trimming, which is what the extra max_chunk - 1 slots hold)."""
 
-    paged = False   # one sequence, as against mimo_moe.paged.PagedKVCache
-
     def __init__(self, cfg: AttentionConfig, cap: int, device=None):
         _no_keep_first(cfg, "KVCache")
         dev = torch.device(device or "cuda")
@@ -229,7 +227,7 @@ class Attention:
     def __call__(self, r: torch.Tensor, cache: KVCache) -> torch.Tensor:
         T = r.shape[0]
         cfg = self.cfg
-        if cache.paged:   # rows of many requests, laid out by the cache's step
+        if getattr(cache, "paged", False):   # rows of many requests, laid out by the cache's step
             return linear(cache.attend(linear(r, self.w_qkv), self.sinks).view(T, -1), self.w_o)
         _no_keep_first(cfg, "attention")
         # the attention call's own check (every key visible to the chunk still in the ring), made before the

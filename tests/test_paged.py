@@ -147,3 +147,14 @@ def test_first_tokens_that_stay_are_refused_before_a_ring_cache_is_touched():
     with pytest.raises(ValueError, match="keep_first"):
         attn(torch.zeros(1, 256, dtype=torch.bfloat16), ring)
     assert ring.offset == 0 and not ring.k.any()
+
+
+def test_a_cache_of_the_callers_own_needs_no_new_attribute():
+    """A layer takes any object with a ring cache's members, as before there were paged ones."""
+    from types import SimpleNamespace
+    from mimo_moe.layer import Attention, AttentionConfig
+    cfg = AttentionConfig(n_heads=2, n_kv_heads=1, head_dim=64, v_head_dim=64, rotary_dim=32)
+    w = torch.zeros(128, 256, dtype=torch.bfloat16)
+    attn = Attention(cfg, w, w[:64], w[:64], w.t())
+    with pytest.raises(ValueError, match="cache slots"):   # the check of the ring's room: past the cache's kind
+        attn(torch.zeros(5, 256, dtype=torch.bfloat16), SimpleNamespace(offset=0, cap=4))
