@@ -17,6 +17,7 @@ The checkpoint's config.json is not available offline, so every dimension is a c
 and 8 on the 128-token sliding-window layers, sinks on the sliding-window layers)."""
 from __future__ import annotations
 
+import struct
 from dataclasses import dataclass, replace
 from functools import lru_cache
 from typing import Optional, Union
@@ -58,10 +59,15 @@ def mimo_sliding_attention(**kw) -> AttentionConfig:
     return replace(AttentionConfig(n_kv_heads=8, rope_theta=10_000.0, window=128, sinks=True), **kw)
 
 
-@lru_cache(maxsize=None)
+@lru_cache(maxsize=64)
+def _bf16_of(bits: bytes) -> float:
+    v = struct.unpack("d", bits)[0]
+    return float(torch.tensor(v, dtype=torch.float32).to(torch.bfloat16).to(torch.float32))
+
+
 def bf16_value(v: float) -> float:
     """The float a Python scalar becomes when MLX multiplies it into a bf16 array (cast to bf16)."""
-    return float(torch.tensor(v, dtype=torch.float32).to(torch.bfloat16).to(torch.float32))
+    return _bf16_of(struct.pack("d", v))   # by its bits: 0.0 and -0.0 are equal, and a scalar tensor may change
 
 
 def _no_keep_first(cfg: AttentionConfig, where: str) -> None:

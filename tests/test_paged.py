@@ -158,3 +158,14 @@ def test_a_cache_of_the_callers_own_needs_no_new_attribute():
     attn = Attention(cfg, w, w[:64], w[:64], w.t())
     with pytest.raises(ValueError, match="cache slots"):   # the check of the ring's room: past the cache's kind
         attn(torch.zeros(5, 256, dtype=torch.bfloat16), SimpleNamespace(offset=0, cap=4))
+
+
+def test_bf16_value_goes_by_the_value_alone():
+    import math
+    from mimo_moe.layer import bf16_value
+    scale = torch.tensor(0.5)
+    assert bf16_value(scale) == 0.5
+    scale.fill_(0.707)
+    assert bf16_value(scale) == bf16_value(0.707) == float(torch.tensor(0.707).to(torch.bfloat16))
+    assert math.copysign(1, bf16_value(0.0)) == 1 and math.copysign(1, bf16_value(-0.0)) == -1
+    assert math.isnan(bf16_value(math.nan)) and bf16_value(1e39) == math.inf and bf16_value(3) == 3.0
