@@ -71,12 +71,14 @@ def _status(device) -> torch.Tensor:
     return torch.zeros(1, dtype=torch.int32, device=device)
 
 
-def read_status(status: torch.Tensor, where: str) -> None:
-    """Synchronise on the status word and raise like the reference does for bad routes."""
+def read_status(status: torch.Tensor, where: str,
+                erange: str = "expert id, more rows than R routed to one expert, or an activation beyond the f16 "
+                              "range") -> None:
+    """Synchronise on the status word and raise like the reference does for bad routes.  erange: what is out of range
+    where the word says that something is."""
     code = int(status.item())
     if code == _lib.MIMO_ERANGE:
-        raise ValueError(f"{where}: value out of range (expert id, more rows than R routed to one "
-                         "expert, or an activation beyond the f16 range)")
+        raise ValueError(f"{where}: value out of range ({erange})")
     if code != _lib.MIMO_OK:
         raise _lib.MimoError(code, where)
 

@@ -65,6 +65,14 @@ def _buffer(t: torch.Tensor, name: str, shape, dev) -> torch.Tensor:
     return t
 
 
+def _check_status(status: torch.Tensor, where: str) -> None:
+    try:
+        read_status(status, where, "no free pages left, a length or a row count that does not fit, or a page or slot "
+                                   "outside the pool")
+    finally:
+        status.zero_()
+
+
 def _page_size(page_size: int) -> int:
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
@@ -124,10 +132,7 @@ class PageStep:
     def check(self, where: str = "paged step") -> None:
         """Synchronise on the status word: ValueError for pages that ran out and lengths or pages that do not fit,
         MimoError for an expired wait.  Clears it."""
-        try:
-            read_status(self.status, where)
-        finally:
-            self.status.zero_()
+        _check_status(self.status, where)
 
 
 def page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -421,10 +426,7 @@ class PagedDecoderStack(DecoderStack):
 
     def check(self) -> None:
         """Synchronise on the status word of the table's steps (PageStep.check)."""
-        try:
-            read_status(self.table.status, "paged stack")
-        finally:
-            self.table.status.zero_()
+        _check_status(self.table.status, "paged stack")
 
     def _result(self, h: torch.Tensor) -> torch.Tensor:
         return self.table._rows.get(("result", h.shape[1]), h.shape[0],

@@ -169,3 +169,22 @@ def test_bf16_value_goes_by_the_value_alone():
     assert bf16_value(scale) == bf16_value(0.707) == float(torch.tensor(0.707).to(torch.bfloat16))
     assert math.copysign(1, bf16_value(0.0)) == 1 and math.copysign(1, bf16_value(-0.0)) == -1
     assert math.isnan(bf16_value(math.nan)) and bf16_value(1e39) == math.inf and bf16_value(3) == 3.0
+
+
+def test_a_step_that_does_not_fit_is_reported_in_its_own_words():
+    from mimo_moe import paged, read_status
+    from mimo_moe._lib import MIMO_ERANGE, MimoError
+    step, stack = object.__new__(paged.PageStep), object.__new__(paged.PagedDecoderStack)
+    stack.table = object.__new__(paged.PageTable)
+    for holder, check in ((step, step.check), (stack.table, stack.check)):
+        holder.status = torch.tensor([MIMO_ERANGE], dtype=torch.int32)
+        with pytest.raises(ValueError, match="page") as e:
+            check()
+        assert "expert" not in str(e.value)
+        check()                                   # cleared
+        holder.status[0] = 5
+        with pytest.raises(MimoError):
+            check()
+        check()
+    with pytest.raises(ValueError, match="expert id"):   # a route's error keeps its words
+        read_status(torch.tensor([MIMO_ERANGE], dtype=torch.int32), "router")
