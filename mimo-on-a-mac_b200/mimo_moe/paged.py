@@ -107,6 +107,7 @@ class PageStep:
         self.status = torch.zeros(1, dtype=torch.int32, device=dev) if status is None else _int32(status, "status",
                                                                                                  (1,), dev)
         self.requests, self.width, self.tokens, self.device = R, block_table.shape[1], T, dev
+        self.version = 0      # how often its lengths were planned anew: an attention plan goes with one of them
         self.rows = _Rows()   # scratch of the layers that work on this step, one after another
 
     @classmethod
@@ -157,6 +158,7 @@ def page_plan(lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Ten
             out.width, free_pages.data_ptr(), n_free.data_ptr(), free_pages.shape[0], out.page_size, tokens,
             out.cu_q.data_ptr(), out.seq_lens.data_ptr(), out.n_free.data_ptr(), out.positions.data_ptr(),
             out.slots.data_ptr(), out.status.data_ptr())
+    out.version += 1
     return out
 
 
@@ -220,6 +222,7 @@ class PageTable:
         self._cu_q = torch.zeros(max_requests + 1, dtype=torch.int32, device=dev)
         self._after = torch.zeros(max_requests + 1, dtype=torch.int32, device=dev)   # the step's lengths and free pages
         self._rows = _Rows()
+        self._step: Optional[PageStep] = None   # the one planned last
 
     def step(self, new_lens: torch.Tensor, tokens: int) -> PageStep:
         """Plan a step (page_plan) and take its lengths and free pages over.  The step's buffers are the table's: the
@@ -236,6 +239,9 @@ class PageTable:
                        slots=self._rows.get("slots", tokens, rows), n_free=self._after[R:], status=self.status)
         out.rows = self._rows
         page_plan(self.lens, new_lens, self.block_table, self.free_pages, self.n_free, self.page_size, tokens, out=out)
+        if self._step is not None:
+            self._step.version += 1   # its buffers are the new step's
+        self._step = out
         self._state.copy_(self._after)
         return out
 
@@ -325,14 +331,16 @@ def _kind(cfg: AttentionConfig):
 
 class AttentionPlan:
     """How attention_paged deals a step's work to the SMs, made from the step's lengths: one for all layers with the
-    same heads, window and keep_first (attention_plan).  It holds until the step's lengths change."""
+    same heads, window and keep_first (attention_plan).  It holds until the step's lengths change: attention_paged refuses
+    it after another page_plan into the step or a later step of the same table, until update().  (A program that writes
+    cu_q or seq_lens itself, or replays a graph that does, calls update() itself.)"""
 
     def __init__(self, step: PageStep, cfg: AttentionConfig):
         if cfg.keep_first and not cfg.window:
             raise ValueError("attention_plan: keep_first needs a window (without one every earlier token is visible)")
         if cfg.n_heads < 1 or cfg.n_kv_heads < 1 or cfg.n_heads % cfg.n_kv_heads or cfg.n_heads // cfg.n_kv_heads > 128:
             raise ValueError(f"attention_plan: {cfg.n_heads} heads over {cfg.n_kv_heads} kv heads")
-        self.step, self.kind = step, _kind(cfg)
+        self.step, self.kind, self.version = step, _kind(cfg), step.version
         self.buffer, self._ws = None, {}
         if step.tokens == 0:
             return
@@ -352,11 +360,11 @@ class AttentionPlan:
     def update(self) -> None:
         """Make the plan again from the step's present lengths, in the same buffer."""
         step, (nq, nkv, window, keep) = self.step, self.kind
-        if self.buffer is None:
-            return
-        _launch(step.device, "attention_plan", lib().mimo_moe_paged_attention_plan, step.cu_q.data_ptr(),
-                step.seq_lens.data_ptr(), step.requests, step.tokens, nq, nkv, window, keep, step.width, step.page_size,
-                self.buffer.data_ptr(), self.buffer.numel(), step.status.data_ptr())
+        if self.buffer is not None:
+            _launch(step.device, "attention_plan", lib().mimo_moe_paged_attention_plan, step.cu_q.data_ptr(),
+                    step.seq_lens.data_ptr(), step.requests, step.tokens, nq, nkv, window, keep, step.width,
+                    step.page_size, self.buffer.data_ptr(), self.buffer.numel(), step.status.data_ptr())
+        self.version = step.version
 
 
 def attention_plan(step: PageStep, cfg: AttentionConfig) -> AttentionPlan:
@@ -386,6 +394,9 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
         plan = AttentionPlan(step, cfg)
     elif plan.step is not step or plan.kind != _kind(cfg):
         raise ValueError("attention_paged: the plan was made for another step or kind of layer")
+    elif plan.version != step.version:
+        raise ValueError("attention_paged: the step's lengths were planned anew since its attention plan was made "
+                         "(plan.update() makes it again)")
     if T == 0:
         return o
     nb = plan.workspace_bytes(cfg.v_head_dim)

@@ -835,3 +835,50 @@ def test_rope_store_paged_refuses_another_clear(gpu):
                                                                              device=gpu)[:, ::2]):
         with pytest.raises(ValueError):
             paged.rope_store_paged(qkv, cfg, cache, step, clear=bad)
+
+
+def test_a_plan_of_earlier_lengths_is_refused_until_it_is_made_again(gpu):
+    """A step planned again in place, and a step whose table has gone on: the attention plan of the lengths before."""
+    from mimo_moe import paged
+    cfg, P, N = cfg_of(D64), 16, 40
+    lens, free = i32([0, 0], gpu), torch.arange(N, dtype=torch.int32, device=gpu)
+    table = torch.full((2, 8), -1, dtype=torch.int32, device=gpu)
+    cache = paged.PagedKVCache(cfg, N, P, gpu)
+    gen = torch.Generator(gpu).manual_seed(3)
+    for t in (cache.k, cache.v):
+        t.copy_(torch.randn(t.shape, generator=gen, device=gpu))
+    q = torch.randn(40, cfg.n_heads, cfg.head_dim, generator=gen, device=gpu).to(torch.bfloat16)
+    step = paged.page_plan(lens, i32([30, 10], gpu), table, free, i32([N], gpu), P, 40)
+    plan = paged.attention_plan(step, cfg)
+    first = paged.attention_paged(q, cache, cfg, step, plan=plan)
+    paged.page_plan(lens, i32([7, 33], gpu), table, free, i32([N], gpu), P, 40, out=step)
+    with pytest.raises(ValueError, match="update"):
+        paged.attention_paged(q, cache, cfg, step, plan=plan)
+    want = paged.attention_paged(q, cache, cfg, step)
+    plan.update()
+    assert torch.equal(paged.attention_paged(q, cache, cfg, step, plan=plan), want) and not torch.equal(first, want)
+    # steps of one table
+    pages = paged.PageTable(2, 128, N, P, gpu)
+    one = pages.step(i32([3, 4], gpu), 7)
+    plan = paged.attention_plan(one, cfg)
+    paged.attention_paged(q[:7], cache, cfg, one, plan=plan)
+    two = pages.step(i32([1, 1], gpu), 7)
+    with pytest.raises(ValueError, match="update"):
+        paged.attention_paged(q[:7], cache, cfg, one, plan=plan)
+    paged.attention_paged(q[:7], cache, cfg, two, plan=paged.attention_plan(two, cfg))
+    none = pages.step(i32([0, 0], gpu), 0)
+    paged.attention_paged(q[:0], cache, cfg, none, plan=paged.attention_plan(none, cfg))
+    # captured: the plan is made again inside the graph, which then serves any lengths
+    new, left = i32([30, 10], gpu), i32([N], gpu)
+    plan = paged.attention_plan(step, cfg)
+    out = torch.zeros(40, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=gpu)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.page_plan(lens, new, table, free, left, P, 40, out=step)
+        plan.update()
+        paged.attention_paged(q, cache, cfg, step, plan=plan, out=out)
+    for lengths, expect in (([30, 10], first), ([7, 33], want)):
+        new.copy_(i32(lengths, gpu))
+        graph.replay()
+        assert torch.equal(out, expect)
+    step.check()
