@@ -126,6 +126,15 @@ __host__ __device__ inline bool whole_units(int tok, int window, int keep) {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kBuckets = 2048;
+// A unit's block count as the sort by length and the CTAs' loads take it: itself below 1024 blocks, above that its first
+// seven significant bits, so that units of one bucket count the same and their order in it, which atomics give, has no say
+// in how the units are dealt.  (A table row of 2^31 positions is 2^24 blocks: bucket 1024 + 14 * 64.)
+__device__ __forceinline__ int bucket_of(int nb) {
+  return nb < 1024 ? nb : 1024 + (int)((__float_as_uint((float)nb) - __float_as_uint(1024.f)) >> 17);
+}
+__device__ __forceinline__ int sorted_as(int nb) {
+  return nb < 1024 ? nb : (int)__uint_as_float(__float_as_uint((float)nb) & ~0x1FFFFu);
+}
 // What a unit costs besides its blocks (Q, the first scores, the epilogue), in blocks.
 constexpr int kUnitCost = 2;
 
@@ -227,7 +236,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
       const int nb = blocks_of(qfirst, qfirst + ntok - 1, p.window, p.keep).n;
       tiles[i] = make_int4(a + t0, ntok, qfirst, r);
       nbs[i] = nb;
-      atomicAdd(&hist[kBuckets - 1 - min(nb, kBuckets - 1)], 1);
+      atomicAdd(&hist[kBuckets - 1 - bucket_of(nb)], 1);
       mine += nb + kUnitCost;
     }
     W = block_scan(mine, &ex, sh);
@@ -252,7 +261,7 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     }
     __syncthreads();
     for (int i = tid; i < nt; i += kPlanThreads)
-      order[atomicAdd(&hist[kBuckets - 1 - min(nbs[i], kBuckets - 1)], 1)] = i;
+      order[atomicAdd(&hist[kBuckets - 1 - bucket_of(nbs[i])], 1)] = i;
     __syncthreads();
   }
   const int units = nt * p.nkv;
@@ -262,7 +271,8 @@ __global__ void __launch_bounds__(kPlanThreads) attn_plan_kernel(AttnPlanParams 
     const int k = u / n, c = u % n;
     return (k & 1) ? n - 1 - c : c;
   };
-  for (int u = tid; u < units; u += kPlanThreads) atomicAdd(&load[cta_of(u)], nbs[order[u / p.nkv]] + kUnitCost);
+  for (int u = tid; u < units; u += kPlanThreads)
+    atomicAdd(&load[cta_of(u)], sorted_as(nbs[order[u / p.nkv]]) + kUnitCost);
   __syncthreads();
   int most = tid < n ? load[tid] : 0;
 #pragma unroll

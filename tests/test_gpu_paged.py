@@ -882,3 +882,27 @@ def test_a_plan_of_earlier_lengths_is_refused_until_it_is_made_again(gpu):
         graph.replay()
         assert torch.equal(out, expect)
     step.check()
+
+
+@pytest.mark.parametrize("blocks", [200, 1500, 2100, 40_000], ids=lambda b: f"{b} blocks")
+def test_how_long_units_are_dealt_goes_by_their_lengths_alone(gpu, blocks):
+    """Whole or split (another order of a row's sum) is the same however often a plan is made and whichever request has
+    which length.  Two units for each SM, 20 of them two blocks longer than the others: a CTA that gets two of the 20 makes
+    splitting worth it, one that gets one does not, so an order that is left to chance shows."""
+    from mimo_moe import paged
+    cfg, P = cfg_of(dict(D64, n_heads=1, n_kv_heads=1)), 128
+    R = 2 * torch.cuda.get_device_properties(gpu).multi_processor_count
+    lens = [128 * (blocks + 2 * (r < 20)) for r in range(R)]
+    table = torch.zeros(R, max(lens) // P, dtype=torch.int32, device=gpu)
+    rng, modes = np.random.default_rng(blocks), []
+    for order in [list(range(R)), list(range(R))[::-1]] + [rng.permutation(R).tolist() for _ in range(16)]:
+        rows = torch.zeros(R, dtype=torch.int32, device=gpu)
+        step = paged.PageStep(block_table=table, page_size=P, cu_q=i32(list(range(R + 1)), gpu),
+                              seq_lens=i32([lens[r] for r in order], gpu), positions=rows, slots=rows)
+        for _ in range(3):
+            plan = paged.attention_plan(step, cfg)
+            head = plan.buffer[:12].view(torch.int32).tolist()
+            assert head[1] == R
+            modes.append(head[2])
+        step.check()
+    assert len(set(modes)) == 1, modes
