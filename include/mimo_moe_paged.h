@@ -13,8 +13,8 @@
  * cache slot is page * page_size + position % page_size.  All layers share one table: a page number names the same
  * positions in every layer's pool.
  *
- * A step has at most 2^30 token rows.  Every pointer is a device pointer, 16-byte aligned where it holds bf16 values.  Errors that the kernels find in
- * device data (MIMO_ERANGE: no free page left, a length outside the table, a page outside the pool) go to the
+ * A step has at most 2^30 token rows, and an attention call 2^30 work units (below).  Every pointer is a device pointer,
+ * 16-byte aligned where it holds bf16 values.  Errors that the kernels find in device data (MIMO_ERANGE: no free page left, a length outside the table, a page outside the pool) go to the
  * optional status word; no device value makes a kernel read or write outside the arrays it is given.
  */
 #ifndef MIMO_MOE_PAGED_H
@@ -79,7 +79,8 @@ int mimo_moe_paged_rope_store_clear(const uint16_t* qkv, int32_t tokens, int32_t
  * anything, NaN included, and table entries of such pages are not read; what one query of a request sees must be finite
  * in v, also for the queries before it.
  *
- * It takes two calls.  The plan deals the step's work to the SMs from its lengths; it holds for all layers with the
+ * It takes two calls.  The plan deals the step's work (units of one kv head of some consecutive tokens of a request) to
+ * the SMs from its lengths; it holds for all layers with the
  * same heads, window and keep_first (a caller-owned buffer, 16-byte aligned, of ..._plan_bytes).  A request whose
  * lengths do not fit (more rows than positions, more positions than its table row, rows outside `tokens`) sets
  * MIMO_ERANGE and gets no output.  The attention must be given the arguments that its plan was made with (otherwise

@@ -1223,6 +1223,11 @@ namespace {
 bool bad_heads(int32_t n_heads, int32_t n_kv_heads) {
   return n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || n_heads / n_kv_heads > 128;
 }
+// (The limit on units is far above any q that fits a GPU; beyond it a plan's 32-bit numbers would overflow.)
+bool bad_step(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads) {
+  return tokens < 1 || tokens > kMaxTokens || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads) ||
+         !attn_units_fit(tokens, R, n_heads / n_kv_heads, n_kv_heads);
+}
 // What a plan depends on besides the lengths themselves, in one word (0 is no plan's).
 int32_t attn_plan_key(int32_t T, int32_t R, int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep,
                       int32_t width, int32_t page_size, int32_t sms) {
@@ -1234,7 +1239,7 @@ int32_t attn_plan_key(int32_t T, int32_t R, int32_t n_heads, int32_t n_kv_heads,
 }  // namespace
 
 size_t mimo_moe_paged_attention_plan_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads) {
-  if (tokens < 1 || tokens > kMaxTokens || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads)) return 0;
+  if (bad_step(tokens, R, n_heads, n_kv_heads)) return 0;
   return attn_plan_bytes(tokens, R, n_heads / n_kv_heads, n_kv_heads, num_sms_current());
 }
 
@@ -1242,7 +1247,7 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
                                   int32_t n_heads, int32_t n_kv_heads, int32_t window, int32_t keep_first,
                                   int32_t table_width, int32_t page_size, void* plan, size_t plan_bytes,
                                   int32_t* status, void* stream) {
-  if (!cu_q || !seq_lens || !plan || tokens < 1 || tokens > kMaxTokens || bad_heads(n_heads, n_kv_heads) || window < 0 || keep_first < 0 ||
+  if (!cu_q || !seq_lens || !plan || bad_step(tokens, R, n_heads, n_kv_heads) || window < 0 || keep_first < 0 ||
       (keep_first > 0 && window == 0) || page_shift_of(page_size) < 0 || bad_table(R, table_width, page_size) ||
       !a16(plan) || plan_bytes < mimo_moe_paged_attention_plan_bytes(tokens, R, n_heads, n_kv_heads))
     return MIMO_EINVAL;
@@ -1258,9 +1263,7 @@ int mimo_moe_paged_attention_plan(const int32_t* cu_q, const int32_t* seq_lens, 
 
 size_t mimo_moe_paged_attention_workspace_bytes(int32_t tokens, int32_t R, int32_t n_heads, int32_t n_kv_heads,
                                                 int32_t v_head_dim) {
-  if (tokens < 1 || tokens > kMaxTokens || R < 1 || R > kMaxRequests || bad_heads(n_heads, n_kv_heads) ||
-      v_head_dim < 1)
-    return 0;
+  if (bad_step(tokens, R, n_heads, n_kv_heads) || v_head_dim < 1) return 0;
   return paged_attn_part_rows(tokens, R, n_heads / n_kv_heads, num_sms_current()) * ((size_t)v_head_dim + 2) * 4;
 }
 
@@ -1270,8 +1273,8 @@ int mimo_moe_paged_attention(const uint16_t* q, const uint16_t* k_pages, const u
                              int32_t window, int32_t keep_first, int32_t num_pages, int32_t page_size,
                              const void* plan, size_t plan_bytes, uint16_t* out, void* workspace,
                              size_t workspace_bytes, int32_t* status, void* stream) {
-  if (!q || !k_pages || !v_pages || !block_table || !plan || !out || !workspace || tokens < 1 ||
-      tokens > kMaxTokens || bad_heads(n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
+  if (!q || !k_pages || !v_pages || !block_table || !plan || !out || !workspace ||
+      bad_step(tokens, R, n_heads, n_kv_heads) || !attn_dims_supported(head_dim, v_head_dim) || !(scale > 0.f) || window < 0 ||
       keep_first < 0 || (keep_first > 0 && window == 0) || bad_pool(num_pages, page_size) ||
       (int64_t)num_pages * n_kv_heads >= INT32_MAX || bad_table(R, table_width, page_size) || !a16(q) ||
       !a16(k_pages) || !a16(v_pages) || !a32(out) || !a16(plan) || !a32(workspace) ||

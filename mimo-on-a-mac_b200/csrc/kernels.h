@@ -371,6 +371,7 @@ struct PagedAttnParams {
   PagedAttnList list[2];         // small units, others
   float scale_log2;              // softmax scale * log2(e)
 };
+bool attn_units_fit(int T, int R, int G, int nkv);  // a step's work units can be numbered in 32 bits
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms);
 size_t paged_attn_part_rows(int T, int R, int G, int num_sms);  // rows of parts a call may write
 cudaError_t launch_attn_plan(AttnPlanParams& p, cudaStream_t st);

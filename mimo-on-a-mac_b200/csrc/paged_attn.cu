@@ -65,6 +65,11 @@ __host__ __device__ inline Lists lists_of(int T, int R, int G) {
   return l;
 }
 
+// Tiles of a list at most: the sum of ceil(n_r / tok) over its requests.
+__host__ __device__ inline int cap_tiles_of(const Lists& ls, int list, int T, int R) {
+  return ls.tok[list] == 0 ? 0 : list == kSmall && !ls.all_small ? R : R + T / ls.tok[list];
+}
+
 // Layout of one list in the plan buffer (32-bit words from its start, every part 16-byte aligned).
 struct PlanLayout {
   int cap_tiles, cap_segs;
@@ -75,10 +80,7 @@ __host__ __device__ inline size_t up4(size_t x) { return (x + 3) & ~(size_t)3; }
 
 __host__ __device__ inline PlanLayout plan_layout(int list, int T, int R, int G, int nkv, int n) {
   PlanLayout L;
-  const Lists ls = lists_of(T, R, G);
-  const int tok = ls.tok[list];
-  // sum of ceil(n_r / tok) over the requests of the list
-  L.cap_tiles = tok == 0 ? 0 : list == kSmall && !ls.all_small ? R : R + T / tok;
+  L.cap_tiles = cap_tiles_of(lists_of(T, R, G), list, T, R);
   L.cap_segs = L.cap_tiles * nkv + n;
   size_t at = 16;  // header: key, units, mode
   L.head = at, at += (size_t)12 * n;  // of each CTA: (its first segment's place, segments), the first segment itself
@@ -1248,6 +1250,13 @@ cudaError_t launch_t(PagedAttnParams& p, int num_sms, cudaStream_t st) {
 }
 
 }  // namespace
+
+bool attn_units_fit(int T, int R, int G, int nkv) {
+  const Lists ls = lists_of(T, R, G);
+  for (int l : {kSmall, kLarge})
+    if ((long long)cap_tiles_of(ls, l, T, R) * nkv > 1 << 30) return false;
+  return true;
+}
 
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms) {
   return 4 * (list_start(kLarge, T, R, G, nkv, num_sms) + plan_layout(kLarge, T, R, G, nkv, num_sms).words);

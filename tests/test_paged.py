@@ -188,3 +188,22 @@ def test_a_step_that_does_not_fit_is_reported_in_its_own_words():
         check()
     with pytest.raises(ValueError, match="expert id"):   # a route's error keeps its words
         read_status(torch.tensor([MIMO_ERANGE], dtype=torch.int32), "router")
+
+
+@pytest.mark.parametrize("T,R,nq,nkv", [(1 << 30, 1, 4096, 4096), (1 << 20, 1, 1 << 20, 1 << 20), (1 << 30, 4096, 2048, 128),
+                                        (4096, 4096, 1 << 30, 1 << 30), (1 << 30, 1, 2**31 - 1, 2**31 - 1)])
+def test_more_work_units_than_32_bits_number_are_refused(T, R, nq, nkv):
+    """Their plan would be written past the bytes that were asked for."""
+    L = _lib()
+    assert L.mimo_moe_paged_attention_plan_bytes(T, R, nq, nkv) == 0
+    assert L.mimo_moe_paged_attention_workspace_bytes(T, R, nq, nkv, 128) == 0
+    assert L.mimo_moe_paged_attention_plan(A, A, R, T, nq, nkv, 0, 0, 8, 16, A, 1 << 60, None, None) == EINVAL
+    assert L.mimo_moe_paged_attention(A, A, A, None, A, 8, R, T, nq, nkv, 192, 128, 0.1, 0, 0, 1, 16, A, 1 << 60, A, A,
+                                      1 << 60, None, None) == EINVAL
+
+
+def test_plan_bytes_grow_with_the_units():
+    L = _lib()
+    for T, R, nq, nkv in ((1 << 30, 1, 64, 4), (1 << 30, 4096, 128, 1), (1 << 20, 4096, 1024, 1024), (4096, 4096, 4096, 4096)):
+        tok = 32 // (nq // nkv) if T <= R else 2 * (128 // (nq // nkv))
+        assert L.mimo_moe_paged_attention_plan_bytes(T, R, nq, nkv) >= 32 * nkv * (T // tok)
