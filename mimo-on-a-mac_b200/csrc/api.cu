@@ -1170,7 +1170,7 @@ int mimo_moe_page_plan(const int32_t* lens, const int32_t* new_lens, int32_t R, 
   p.cu_q = cu_q, p.seq_lens = seq_lens, p.n_free_out = n_free_out, p.positions = positions, p.slots = slots;
   p.status = status, p.R = R, p.width = table_width, p.num_pages = num_pages, p.page_shift = page_shift_of(page_size);
   p.tokens = tokens;
-  MIMO_TRY(launch_page_plan(p, static_cast<cudaStream_t>(stream)));
+  MIMO_TRY(launch_page_plan(p, num_sms_current(), static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
 }
 
@@ -1205,7 +1205,7 @@ int mimo_moe_paged_rope_store_clear(const uint16_t* qkv, int32_t tokens, int32_t
   p.T = tokens, p.nq = n_heads, p.nkv = n_kv_heads, p.dqk = head_dim, p.dv = v_head_dim, p.rot = rotary_dim;
   p.num_pages = num_pages, p.page_shift = page_shift_of(page_size), p.has_vscale = v_scale > 0.f ? 1 : 0;
   p.v_scale = v_scale, p.log_base = std::log((double)rope_theta);
-  MIMO_TRY(launch_paged_rope(p, static_cast<cudaStream_t>(stream)));
+  MIMO_TRY(launch_paged_rope(p, num_sms_current(), static_cast<cudaStream_t>(stream)));
   return MIMO_OK;
 }
 

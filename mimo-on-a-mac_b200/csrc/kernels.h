@@ -375,9 +375,9 @@ bool attn_units_fit(int T, int R, int G, int nkv);  // a step's work units can b
 size_t attn_plan_bytes(int T, int R, int G, int nkv, int num_sms);
 size_t paged_attn_part_rows(int T, int R, int G, int num_sms);  // rows of parts a call may write
 cudaError_t launch_attn_plan(AttnPlanParams& p, cudaStream_t st);
-cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st);
+cudaError_t launch_page_plan(const PagePlanParams& p, int num_sms, cudaStream_t st);
 cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st);
-cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st);
+cudaError_t launch_paged_rope(const PagedRopeParams& p, int num_sms, cudaStream_t st);
 cudaError_t launch_paged_attention(PagedAttnParams& p, int num_sms, cudaStream_t st);
 
 }  // namespace mimo

@@ -376,9 +376,9 @@ __global__ void __launch_bounds__(kRopeThreads) paged_rope_kernel(PagedRopeParam
 
 }  // namespace
 
-cudaError_t launch_page_plan(const PagePlanParams& p, cudaStream_t st) {
+cudaError_t launch_page_plan(const PagePlanParams& p, int num_sms, cudaStream_t st) {
   // a row a thread: the searches and the table entry are latency, the scan that every CTA repeats is small beside them
-  const int blocks = std::max(1, std::min(148, (p.tokens + kPlanThreads - 1) / kPlanThreads));
+  const int blocks = std::max(1, std::min(num_sms, (p.tokens + kPlanThreads - 1) / kPlanThreads));
   return launch_k(page_plan_kernel, dim3(blocks), dim3(kPlanThreads), (size_t)(2 * p.R + 2) * 4, st, p);
 }
 
@@ -388,7 +388,7 @@ cudaError_t launch_page_release(const PageReleaseParams& p, cudaStream_t st) {
 
 namespace {
 template <int THREADS>
-cudaError_t launch_rope_rows(const PagedRopeParams& p, size_t smem, int fit, cudaStream_t st) {
+cudaError_t launch_rope_rows(const PagedRopeParams& p, size_t smem, int most, cudaStream_t st) {
   static bool attr_set[128] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -398,23 +398,24 @@ cudaError_t launch_rope_rows(const PagedRopeParams& p, size_t smem, int fit, cud
     if (e != cudaSuccess) return e;
     attr_set[dev] = true;
   }
-  const int most = 148 * fit, rounds = (p.T + most - 1) / most;  // all CTAs have the same number of rows, or one less
+  const int rounds = (p.T + most - 1) / most;  // all CTAs have the same number of rows, or one less
   return launch_k(paged_rope_rows_kernel<THREADS>, dim3((p.T + rounds - 1) / rounds), dim3(THREADS), smem, st, p);
 }
 }  // namespace
 
-cudaError_t launch_paged_rope(const PagedRopeParams& p, cudaStream_t st) {
+cudaError_t launch_paged_rope(const PagedRopeParams& p, int num_sms, cudaStream_t st) {
   const size_t smem = kRowHead + ((size_t)(p.nq + p.nkv) * p.dqk + (size_t)p.nkv * p.dv) * 2;
   if (p.rot % 16 == 0 && smem <= kRowSmem) {
     const int fit = (int)std::min<size_t>(16, (228 * 1024) / (smem + 1024));  // CTAs an SM
     // A CTA of 128 threads keeps up with memory where several rows of an SM are worked on at once; alone, 384 threads are
     // through its row sooner (8 rows of 64 + 4 heads: 2.6 us against 2.9; 16000 of 32 + 8 heads of 128 with 256 threads:
     // 105 us against 79, as fewer CTAs fit).
-    return p.T <= 148 || fit < 3 ? launch_rope_rows<384>(p, smem, fit, st) : launch_rope_rows<128>(p, smem, fit, st);
+    return p.T <= num_sms || fit < 3 ? launch_rope_rows<384>(p, smem, num_sms * fit, st)
+                                     : launch_rope_rows<128>(p, smem, num_sms * fit, st);
   }
   // shares of a row down to a value a thread while there are fewer rows than four for each SM
   const int all = (p.nq + p.nkv) * (p.dqk - p.rot / 2) + p.nkv * p.dv;
-  const int shares = std::max(1, std::min((all + kRopeThreads - 1) / kRopeThreads, 4 * 148 / p.T));
+  const int shares = std::max(1, std::min((all + kRopeThreads - 1) / kRopeThreads, 4 * num_sms / p.T));
   return launch_k(paged_rope_kernel, dim3(p.T, shares), dim3(kRopeThreads), 0, st, p);
 }
 
