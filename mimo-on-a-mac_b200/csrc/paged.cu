@@ -260,11 +260,7 @@ __global__ void __launch_bounds__(THREADS) paged_rope_rows_kernel(PagedRopeParam
   for (; t < p.T; t += gridDim.x) {
     const int my_slot = slot, my_pos = pos;
     if (t + (int)gridDim.x < p.T) slot = p.slots[t + gridDim.x], pos = p.positions[t + gridDim.x];
-    if (my_slot < 0) {
-      if (p.clear != nullptr)
-        for (int i = tid; i < p.clear_n; i += THREADS) p.clear[(size_t)t * p.clear_n + i] = make_uint4(0, 0, 0, 0);
-      continue;
-    }
+    if (my_slot < 0) continue;
     if (tid < 32) {
       asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory");  // the row before has left
       __syncwarp();
@@ -321,6 +317,11 @@ __global__ void __launch_bounds__(THREADS) paged_rope_rows_kernel(PagedRopeParam
       asm volatile("cp.async.bulk.commit_group;\n" ::: "memory");
     }
   }
+  // (in a loop of its own: a branch in the one above made 2048 rows 22.4 us instead of 21.7)
+  if (p.clear != nullptr)
+    for (t = blockIdx.x; t < p.T; t += gridDim.x)
+      if (p.slots[t] < 0)
+        for (int i = tid; i < p.clear_n; i += THREADS) p.clear[(size_t)t * p.clear_n + i] = make_uint4(0, 0, 0, 0);
   if (tid < 32) asm volatile("cp.async.bulk.wait_group 0;\n" ::: "memory");
 }
 

@@ -312,15 +312,17 @@ def rope_store_paged(qkv: torch.Tensor, cfg: AttentionConfig, cache: PagedKVCach
     qkv = _bf16(qkv, "qkv", (T, cfg.qkv_width), dev)
     shape = (T, cfg.n_heads, cfg.head_dim)
     q = torch.empty(shape, dtype=torch.bfloat16, device=dev) if q_out is None else _buffer(q_out, "q_out", shape, dev)
+    entry, more = lib().mimo_moe_paged_rope_store, ()
     if clear is not None:
         _buffer(clear, "clear", (T, cfg.n_heads, cfg.v_head_dim), dev)
+        entry, more = lib().mimo_moe_paged_rope_store_clear, (clear.data_ptr(), cfg.n_heads * cfg.v_head_dim)
     if T == 0:
         return q
     vs = 0.0 if cfg.v_scale is None else bf16_value(cfg.v_scale)
-    _launch(dev, "rope_store_paged", lib().mimo_moe_paged_rope_store_clear, qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads,
+    _launch(dev, "rope_store_paged", entry, qkv.data_ptr(), T, cfg.n_heads, cfg.n_kv_heads,
             cfg.head_dim, cfg.v_head_dim, cfg.rotary_dim, cfg.rope_theta, vs, step.positions.data_ptr(),
             step.slots.data_ptr(), cache.num_pages, cache.page_size, q.data_ptr(), cache.k.data_ptr(),
-            cache.v.data_ptr(), _ptr(clear), cfg.n_heads * cfg.v_head_dim, step.status.data_ptr())
+            cache.v.data_ptr(), *more, step.status.data_ptr())
     return q
 
 
