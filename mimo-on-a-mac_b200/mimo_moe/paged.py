@@ -283,6 +283,7 @@ class PagedKVCache:
         step, cfg = self.step, self.cfg
         if step is None:
             raise ValueError("PagedKVCache: no step set (cache.step = table.step(new_lens, tokens))")
+        _fits(self, cfg, step, "PagedKVCache")   # before the scratch is made on this cache's device
 
         def rows(n):
             return torch.zeros(n, cfg.n_heads, cfg.v_head_dim, dtype=torch.bfloat16, device=self.device)

@@ -207,3 +207,18 @@ def test_plan_bytes_grow_with_the_units():
     for T, R, nq, nkv in ((1 << 30, 1, 64, 4), (1 << 30, 4096, 128, 1), (1 << 20, 4096, 1024, 1024), (4096, 4096, 4096, 4096)):
         tok = 32 // (nq // nkv) if T <= R else 2 * (128 // (nq // nkv))
         assert L.mimo_moe_paged_attention_plan_bytes(T, R, nq, nkv) >= 32 * nkv * (T // tok)
+
+
+def test_a_refused_layer_call_leaves_no_buffer_behind():
+    """A cache that does not go with the step (another device, other pages) is refused before the step's scratch is made:
+    a buffer of it, on the cache's device, would be what the next layer is given."""
+    from mimo_moe import paged
+    from mimo_moe.layer import AttentionConfig
+    step = object.__new__(paged.PageStep)
+    step.rows, step.tokens, step.page_size, step.device = paged._Rows(), 4, 16, torch.device("cuda", 0)
+    cache = object.__new__(paged.PagedKVCache)
+    cache.cfg, cache.page_size, cache.num_pages, cache.device = AttentionConfig(), 16, 8, torch.device("cpu")
+    cache.step, cache.plan = step, None
+    with pytest.raises(ValueError, match="pages of 16 on cpu"):
+        cache.attend(torch.zeros(4, cache.cfg.qkv_width), None)
+    assert not step.rows._bufs
