@@ -77,7 +77,8 @@ int mimo_moe_paged_rope_store_clear(const uint16_t* qkv, int32_t tokens, int32_t
  * not null.  q bf16 [tokens][n_heads][head_dim], out bf16 [tokens][n_heads][v_head_dim]; (head_dim, v_head_dim) in
  * {(192,128), (128,128), (64,64)}; n_heads / n_kv_heads <= 128.  Cache slots that no query of the call sees may hold
  * anything, NaN included, and table entries of such pages are not read; what one query of a request sees must be finite
- * in v, also for the queries before it.
+ * in v, also for the queries before it, and below 2^40 in magnitude (a row's exponentials, before they are divided by
+ * their sum, may be as large as 2^60).
  *
  * It takes two calls.  The plan deals the step's work (units of one kv head of some consecutive tokens of a request) to
  * the SMs from its lengths; it holds for all layers with the

@@ -226,8 +226,8 @@ __device__ __forceinline__ uint32_t scaled(uint32_t w, float s) {
 // Whole token rows through shared memory, in CTAs that each hold one: a row of projections comes in with one bulk copy,
 // its rotary pairs and values are rotated and scaled in place while other CTAs' rows are on their way, and it goes out
 // with one bulk copy for q (the row's q heads lie as they do in the input) and one for each kv head's k and v.  What is in
-// flight costs no registers: six rows of 27 KB an SM.  2048 rows of 64 + 4 heads of 192 are 111 MB and take 22.8 us (4.9
-// TB/s; 32 through registers), 16000 of them 154 us (5.6 TB/s; 198), 8 rows 2.6 us (2.7).
+// flight costs no registers: six rows of 27 KB an SM.  2048 rows of 64 + 4 heads of 192 are 111 MB and take 21.8 us (5.1
+// TB/s; 32 through registers), 16000 of them 153 us (5.7 TB/s; 198), 8 rows 2.6 us (2.7).
 constexpr size_t kRowSmem = 232448;  // a CTA's most
 constexpr int kRowHead = 128 * 16 + 128 * 8 + 128;  // cosines and sines, frequencies, the barrier
 

@@ -381,7 +381,8 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, cfg: AttentionConfig, 
     """mimo_moe.layer.attention for a step's token rows over the paged cache: causal; with cfg.window a sliding window,
     in which each request's first cfg.keep_first tokens stay visible; sinks float32 [n_heads].  plan: the step's
     attention_plan for this kind of layer (made for this call when None).  Cache slots that no query of the step sees
-    may hold anything; v at a position that one query sees must be finite for the request's earlier queries too.
+    may hold anything; v at a position that one query sees must be finite for the request's earlier queries too, and
+    below 2^40 in magnitude.
     Returns bf16 [tokens, n_heads, v_head_dim]; padding rows of a given `out` are not written, those of a new one are
     zero."""
     _fits(cache, cfg, step, "attention_paged")
@@ -417,7 +418,8 @@ class PagedDecoderStack(DecoderStack):
     new_lens int32 [max_requests]) plans the step, runs the layers and returns the rows' hidden states (a buffer of the
     stack's, which the next call writes again); the lengths advance on the device, so a decode step captured once as a
     CUDA graph serves the tokens that follow as well.  `release(done)` frees finished requests' rows; `check()` raises
-    when a step could not be planned (it then ran without new tokens).  Padding rows of x need only be finite."""
+    when a step could not be planned (it then ran without new tokens).  Padding rows of x need only be finite.  One table
+    serves all layers, so sliding-window layers hold every token of a request too, not a window of them."""
 
     def __init__(self, layers, max_requests: int, max_len: int, num_pages: int, page_size: int = 64):
         if not layers:
